@@ -334,6 +334,94 @@ int rl_hip_argmax_rows(const float* logits, int rows, int vocab, int* out_idx, f
 int rl_hip_accept_prefix(const int* toks, const int* preds, int T, int* pos, int* n_consumed, int* next_tok,
                          void* stream);
 
+/* ---- paged KV cache: append, attention of drafted trees, tree acceptance ------
+ * No counterpart in the reference (its cache is one run of positions per sequence and
+ * its drafts are a chain); the serving form of rl_hip_attn_decode_layer and
+ * rl_hip_accept_prefix.  One step: rl_hip_paged_append writes the step's K / V,
+ * rl_hip_tree_attn attends, rl_hip_sample_rows picks every row's next token,
+ * rl_hip_tree_accept keeps the accepted path.
+ *
+ * A step's tokens are "rows", sequence after sequence: sequence b has rows
+ * row_start[b] .. row_start[b+1]-1 (device, n_seq + 1 ints, non-decreasing; rows from
+ * row_start[n_seq] on belong to none and their outputs are left as they were), a
+ * context of ctx_lens[b] positions, and its row j sits at position ctx_lens[b] + j of
+ * its page table (entry p / page_size of row b of `table` [n_seq][table_width]; entries
+ * past the sequence's last position are not read).
+ * `dtype` is the rows' type: RL_Q_F32 (over an RL_Q_F16 cache) or the cache's own.
+ * Lengths, tables and slots are read on the device, so a captured call follows them;
+ * page numbers and slots outside the cache are never accessed. */
+
+/* Rows of q, k and v (head h of row i at q + i * q_row + h * q_head elements, likewise k
+ * and v; pointers aligned to four elements, strides multiples of 4): RMSNorm per head
+ * with weight 1 + q_norm / 1 + k_norm (NULL: weight 1) unless use_norm is 0, rotate-half
+ * RoPE over the first rotary_dim dims (a multiple of 8, 0: none) at position pos[i] with
+ * frequencies theta^(-2 j / rotary_dim) (angles in 64 bits), then q to q_out
+ * [rows][n_q][head_dim] and k, v to slot slots[i] (page * page_size + row of the page) of
+ * `layer`.  A row whose slot is negative or past the last page leaves the cache as it
+ * is; two rows must not have one slot.  q_out must not overlap the inputs.  n_q = 0:
+ * keys and values only. */
+int rl_hip_paged_append(const RlPagedCache* cache, int layer, int dtype, const void* q, int64_t q_row, int64_t q_head,
+                        const void* k, int64_t k_row, int64_t k_head, const void* v, int64_t v_row, int64_t v_head,
+                        const float* q_norm, const float* k_norm, int use_norm, float eps, int rotary_dim, float theta,
+                        const int* pos, const int64_t* slots, int rows, int n_q, void* q_out, void* stream);
+
+/* out [rows][n_q][head_dim] = softmax(scale q . K^T) V, times sigmoid(gate) where gate is
+ * given (addressed as q).  Row j of a sequence sees the whole context and, of the
+ * sequence's rows, those with their bit set in mask [rows][mask_words] (row i at bit
+ * i % 64 of word i / 64; its own bit included or not as the caller wants; rows past the
+ * words are not seen), or rows 0 .. j where mask is NULL.  A row that sees nothing gets
+ * zeros; what a row does not see does not reach it, infinities and NaN included.  n_q a
+ * multiple of n_kv with at most 64 query heads per kv head; max_rows: no sequence has
+ * more rows (rows past it are left out).  A context that with its rows passes the table
+ * is cut to what the table holds; a page number outside the cache is read as page 0.
+ * q and gate aligned and strided as in rl_hip_paged_append; out 16-byte aligned.
+ * workspace: rl_hip_tree_attn_workspace_bytes; calls that overlap in time need one each. */
+size_t rl_hip_tree_attn_workspace_bytes(int n_q, int n_kv, int head_dim, int n_seq, int max_rows);
+int rl_hip_tree_attn(const RlPagedCache* cache, int layer, int dtype, const void* q, int64_t q_row, int64_t q_head,
+                     const void* gate, int64_t gate_row, int64_t gate_head, const int* table, int table_width,
+                     const int* ctx_lens, const int* row_start, int n_seq, int rows, int max_rows,
+                     const uint64_t* mask, int mask_words, int n_q, float scale, void* out, void* workspace,
+                     size_t workspace_bytes, void* stream);
+
+/* Greedy walk through every sequence's tree: from its row 0 (the root) to the first row
+ * (lowest index) whose parent is the current row and whose token is the current row's
+ * sample, until there is none or path_cap rows are on the path.  parents [rows]: row
+ * number within the sequence, lower than the row's own (others have no parent).
+ * path [n_seq][path_cap] gets the rows of the path, then -1; n_accept its length (0 for
+ * a sequence without rows), next_tok the last one's sample (-1), ctx_out
+ * ctx_lens + n_accept (not the same memory as ctx_lens).  In every layer of the cache
+ * (NULL: none) the K and V of path row d move to position ctx_lens[b] + d, so that the
+ * path follows the context; positions behind it keep what they held.  Two sequences must
+ * not share a page that holds rows of this step. path_cap <= 4096. */
+int rl_hip_tree_accept(const RlPagedCache* cache, const int* table, int table_width, const int* ctx_lens,
+                       const int* row_start, int n_seq, int rows, const int* parents, const int* toks,
+                       const int* samples, int* path, int path_cap, int* n_accept, int* next_tok, int* ctx_out,
+                       void* stream);
+
+/* ---- sampling -----------------------------------------------------------------
+ * The sampled form of rl_hip_argmax_rows (the reference samples greedily only): one
+ * token for each of `rows` rows of logits [rows][ld] (type RL_Q_F32, RL_Q_F16 or
+ * RL_Q_BF16; ld >= vocab) from the caller's uniform numbers u [rows] in [0, 1).
+ * With weights exp((logit - row maximum) / temperature):
+ *   top_k   keeps the k largest (equal ones by lowest index; <= 0 or >= vocab: all),
+ *   top_p   of those, in that order, the ones before which less than top_p of their
+ *           total stands (at least one; >= 1 or NaN: all),
+ *   min_p   of those, the ones whose weight is at least min_p (values above 1 count as
+ *           1; <= 0 or NaN: all),
+ * then the token is the first, by index, up to which more than u of what is left
+ * stands; out_prob (may be NULL) is its share of what is left.  temperature <= 0 or NaN:
+ * the argmax, with probability 1.  Each of the four arrays may be NULL (1, 0, 1, 0).
+ * NaN logits are never picked; a row without a logit above -infinity gives token 0 with
+ * probability 0; among logits of +infinity the weights are 1 and all others 0.
+ * Weights are sums of integers, in units of at most 2^-44 of the largest up to a vocab of
+ * 2^18 (above, vocab * 2^-62), so the result does not depend on the order of the work;
+ * tokens below half a unit are never picked.  vocab <= 2^24.  workspace:
+ * rl_hip_sample_workspace_bytes; calls that overlap in time need one each. */
+size_t rl_hip_sample_workspace_bytes(int rows, int vocab);
+int rl_hip_sample_rows(int dtype, const void* logits, int64_t ld, int rows, int vocab, const float* temperature,
+                       const int* top_k, const float* top_p, const float* min_p, const float* u, int* out_idx,
+                       float* out_prob, void* workspace, size_t workspace_bytes, void* stream);
+
 /* ---- decode engine ----------------------------------------------------------
  * Replaces: cuda_gen::Engine (include/rapidllm/runtime/cuda_engine.h:13-83) and its
  * CUDA implementation's decode / verify / MTP paths (src/kernels/cuda/cuda_engine.cu:

@@ -68,6 +68,20 @@ typedef struct RlTensor {
     const float* scale; /* FP8 block scales, NULL otherwise */
 } RlTensor;
 
+/*
+ * A KV cache in pages: k and v, each [n_layers][n_pages][n_kv][page_size][head_dim] of
+ * `dtype` (RL_Q_F16 or RL_Q_BF16), layers layer_stride elements apart.  A sequence's
+ * position p is row p % page_size of page table[p / page_size] of its page table.
+ * head_dim 64, 128 or 256; page_size a power of two up to 4096; k and v 16-byte
+ * aligned, layer_stride a multiple of 8.
+ */
+typedef struct RlPagedCache {
+    void* k;
+    void* v;
+    int64_t layer_stride;
+    int n_layers, n_pages, page_size, n_kv, head_dim, dtype;
+} RlPagedCache;
+
 #ifdef __cplusplus
 }
 #endif

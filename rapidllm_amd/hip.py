@@ -18,6 +18,16 @@ _vp = C.c_void_p
 _sz = C.c_size_t
 _i = C.c_int
 
+
+class RlPagedCache(C.Structure):
+    """include/rl_model.h: a KV cache in pages."""
+    _fields_ = [("k", _vp), ("v", _vp), ("layer_stride", C.c_int64), ("n_layers", _i), ("n_pages", _i),
+                ("page_size", _i), ("n_kv", _i), ("head_dim", _i), ("dtype", _i)]
+
+
+_pc = C.POINTER(RlPagedCache)
+_i64 = C.c_int64
+
 # name -> (restype, argtypes); every entry point returns an RlStatus unless noted.
 _SIGS = {
     "rl_hip_abi_version": (_i, []),
@@ -83,6 +93,14 @@ _SIGS = {
     "rl_hip_argmax_workspace_bytes": (_sz, [_i, _i]),
     "rl_hip_argmax_rows": (_i, [_vp, _i, _i, _vp, _vp, _vp, _vp]),
     "rl_hip_accept_prefix": (_i, [_vp, _vp, _i, _vp, _vp, _vp, _vp]),
+    "rl_hip_paged_append": (_i, [_pc, _i, _i, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _i,
+                                 C.c_float, _i, C.c_float, _vp, _vp, _i, _i, _vp, _vp]),
+    "rl_hip_tree_attn_workspace_bytes": (_sz, [_i, _i, _i, _i, _i]),
+    "rl_hip_tree_attn": (_i, [_pc, _i, _i, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i, _vp, _vp, _i, _i, _i, _vp, _i,
+                              _i, C.c_float, _vp, _vp, _sz, _vp]),
+    "rl_hip_tree_accept": (_i, [_pc, _vp, _i, _vp, _vp, _i, _i, _vp, _vp, _vp, _vp, _i, _vp, _vp, _vp, _vp]),
+    "rl_hip_sample_workspace_bytes": (_sz, [_i, _i]),
+    "rl_hip_sample_rows": (_i, [_i, _vp, _i64, _i, _i, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
     "rl_hip_engine_create": (_vp, [_vp, _vp, _i, _i, _i, C.POINTER(_i)]),
     "rl_hip_engine_create_synthetic": (_vp, [_vp, C.c_uint64, _i, _i, C.POINTER(_i)]),
     "rl_hip_engine_destroy": (None, [_vp]),

@@ -416,6 +416,116 @@ def attn_prefill_layer(Y, cache: AttnCache, pos: int, q_norm, k_norm, n_q, n_kv,
     return d_out.numpy(np.float32, (T, n_q * hd))
 
 
+# ------------------------------------------------------------------ paged cache
+
+F32, F16, BF16 = 0, 1, 2  # RlQuant values
+
+
+def row_bits(a, dtype: int) -> np.ndarray:
+    """float values as rows of `dtype` (rounded to nearest even; BF16 as uint16 bits)."""
+    a = _f32(a)
+    if dtype == F32:
+        return a
+    if dtype == F16:
+        with np.errstate(over="ignore"):
+            return a.astype(np.float16)
+    u = a.view(np.uint32)
+    r = ((u + 0x7FFF + ((u >> 16) & 1)) >> 16).astype(np.uint16)
+    return np.where(np.isnan(a), np.uint16(0x7FC0), r)
+
+
+def row_values(a: np.ndarray, dtype: int) -> np.ndarray:
+    """The fp32 values of row_bits."""
+    if dtype == BF16:
+        return (a.astype(np.uint32) << 16).view(np.float32)
+    return a.astype(np.float32)
+
+
+def _row_np(dtype):
+    return {F32: np.float32, F16: np.float16, BF16: np.uint16}[dtype]
+
+
+class PagedCache:
+    """K and V pages in HBM, [layers][pages][n_kv][page_size][head_dim] each
+    (include/rl_model.h, RlPagedCache)."""
+
+    def __init__(self, n_pages: int, page_size: int, n_kv: int, head_dim: int, dtype: int = F16, n_layers: int = 1):
+        self.shape = (n_layers, n_pages, n_kv, page_size, head_dim)
+        n = int(np.prod(self.shape))
+        self.k, self.v = DeviceBuffer(2 * n), DeviceBuffer(2 * n)
+        self.k.zero()
+        self.v.zero()
+        call("rl_hip_device_synchronize")
+        self.desc = hip.RlPagedCache(self.k.ptr, self.v.ptr, n // n_layers, n_layers, n_pages, page_size, n_kv,
+                                     head_dim, dtype)
+
+    def fill(self, K, V):
+        """K, V: float values in the cache's shape."""
+        for buf, a in ((self.k, K), (self.v, V)):
+            buf.upload(row_bits(np.asarray(a).reshape(self.shape), self.desc.dtype))
+
+    def values(self):
+        """(K, V) as fp32 arrays in the cache's shape."""
+        t = self.desc.dtype
+        return tuple(row_values(b.numpy(_row_np(t), self.shape), t) for b in (self.k, self.v))
+
+
+def paged_append(cache: PagedCache, layer: int, q, k, v, pos, slots, q_norm=None, k_norm=None, norm=True, eps=1e-6,
+                 rotary_dim=64, theta=1e7, dtype: int = F32, stream=None) -> np.ndarray:
+    """q [rows][n_q][hd], k and v [rows][n_kv][hd] (float values): normed and rotated q
+    back, k and v in the cache at `slots`."""
+    n, nq, hd = np.shape(q)
+    bufs = [DeviceBuffer.from_numpy(row_bits(a, dtype)) for a in (q, k, v)]
+    g = [DeviceBuffer.from_numpy(_f32(a)) if a is not None else None for a in (q_norm, k_norm)]
+    d_pos = DeviceBuffer.from_numpy(np.asarray(pos, np.int32))
+    d_slots = DeviceBuffer.from_numpy(np.asarray(slots, np.int64))
+    out = DeviceBuffer(bufs[0].nbytes)
+    nkv = np.shape(k)[1]
+    call("rl_hip_paged_append", cache.desc, layer, dtype, bufs[0].ptr, nq * hd, hd, bufs[1].ptr, nkv * hd, hd,
+         bufs[2].ptr, nkv * hd, hd, g[0].ptr if g[0] else None, g[1].ptr if g[1] else None, 1 if norm else 0, eps,
+         rotary_dim, theta, d_pos.ptr, d_slots.ptr, n, nq, out.ptr, stream)
+    call("rl_hip_stream_synchronize", stream)
+    return row_values(out.numpy(_row_np(dtype), (n, nq, hd)), dtype)
+
+
+def tree_attn(cache: PagedCache, layer: int, q, table, ctx_lens, row_start, mask=None, gate=None, scale=None,
+              dtype: int = F32, max_rows=None, out0=None, stream=None) -> np.ndarray:
+    """Attention of rows q [rows][n_q][hd] over their sequences' pages; mask [rows][words]
+    uint64 or None (causal).  out0: what the output buffer holds before the call."""
+    n, nq, hd = np.shape(q)
+    table = np.ascontiguousarray(table, np.int32)
+    B, width = table.shape
+    if max_rows is None:
+        max_rows = int(np.max(np.diff(row_start), initial=0))
+    d_q = DeviceBuffer.from_numpy(row_bits(q, dtype))
+    d_g = DeviceBuffer.from_numpy(row_bits(gate, dtype)) if gate is not None else None
+    d_t, d_c, d_r = (DeviceBuffer.from_numpy(np.asarray(a, np.int32)) for a in (table, ctx_lens, row_start))
+    d_m = DeviceBuffer.from_numpy(np.asarray(mask, np.uint64)) if mask is not None else None
+    d_o = DeviceBuffer.from_numpy(row_bits(np.zeros((n, nq, hd)) if out0 is None else out0, dtype))
+    nkv = cache.desc.n_kv
+    ws = DeviceBuffer(hip.lib().rl_hip_tree_attn_workspace_bytes(nq, nkv, hd, B, max_rows))
+    call("rl_hip_tree_attn", cache.desc, layer, dtype, d_q.ptr, nq * hd, hd, d_g.ptr if d_g else None, nq * hd, hd,
+         d_t.ptr, width, d_c.ptr, d_r.ptr, B, n, max_rows, d_m.ptr if d_m else None,
+         np.shape(mask)[1] if mask is not None else 0, nq, 1.0 / np.sqrt(hd) if scale is None else scale, d_o.ptr,
+         ws.ptr, ws.nbytes, stream)
+    call("rl_hip_stream_synchronize", stream)
+    return row_values(d_o.numpy(_row_np(dtype), (n, nq, hd)), dtype)
+
+
+def tree_accept(cache, table, ctx_lens, row_start, parents, toks, samples, path_cap: int, stream=None):
+    """Accepted path of every sequence's tree; moves its K / V behind the context in
+    `cache` (or None).  Returns (path [n_seq][path_cap], n_accept, next_tok, ctx_out)."""
+    B = len(ctx_lens)
+    ins = [DeviceBuffer.from_numpy(np.asarray(a, np.int32)) for a in (ctx_lens, row_start, parents, toks, samples)]
+    d_t = DeviceBuffer.from_numpy(np.ascontiguousarray(table, np.int32)) if table is not None else None
+    outs = [DeviceBuffer(4 * B * path_cap), DeviceBuffer(4 * B), DeviceBuffer(4 * B), DeviceBuffer(4 * B)]
+    call("rl_hip_tree_accept", cache.desc if cache else None, d_t.ptr if d_t else None,
+         np.shape(table)[1] if table is not None else 0, ins[0].ptr, ins[1].ptr, B, len(parents), ins[2].ptr,
+         ins[3].ptr, ins[4].ptr, outs[0].ptr, path_cap, outs[1].ptr, outs[2].ptr, outs[3].ptr, stream)
+    call("rl_hip_stream_synchronize", stream)
+    return (outs[0].numpy(np.int32, (B, path_cap)), *(o.numpy(np.int32, (B,)) for o in outs[1:]))
+
+
 # ------------------------------------------------------------------ sampling
 
 
@@ -429,6 +539,27 @@ def argmax_rows(logits: np.ndarray):
     ws = DeviceBuffer(hip.lib().rl_hip_argmax_workspace_bytes(rows, V))
     call("rl_hip_argmax_rows", d_l.ptr, rows, V, d_i.ptr, d_v.ptr, ws.ptr, None)
     return d_i.numpy(np.int32, (rows,)), d_v.numpy(np.float32, (rows,))
+
+
+def sample_rows(logits, u, temperature=None, top_k=None, top_p=None, min_p=None, dtype: int = F32, ld=None,
+                stream=None):
+    """One token per row of logits [rows][vocab] from uniform numbers u: (tokens, their
+    probabilities).  The settings are per row or None."""
+    logits = np.atleast_2d(np.asarray(logits, np.float32))
+    rows, V = logits.shape
+    ld = ld or V
+    padded = np.zeros((rows, ld), np.float32)
+    padded[:, :V] = logits
+    d_l = DeviceBuffer.from_numpy(row_bits(padded, dtype))
+    d_u = DeviceBuffer.from_numpy(_f32(u))
+    par = [None if a is None else DeviceBuffer.from_numpy(np.ascontiguousarray(np.broadcast_to(a, (rows,)), t))
+           for a, t in ((temperature, np.float32), (top_k, np.int32), (top_p, np.float32), (min_p, np.float32))]
+    d_i, d_p = DeviceBuffer(4 * rows), DeviceBuffer(4 * rows)
+    ws = DeviceBuffer(hip.lib().rl_hip_sample_workspace_bytes(rows, V))
+    call("rl_hip_sample_rows", dtype, d_l.ptr, ld, rows, V, *[b.ptr if b else None for b in par], d_u.ptr, d_i.ptr,
+         d_p.ptr, ws.ptr, ws.nbytes, stream)
+    call("rl_hip_stream_synchronize", stream)
+    return d_i.numpy(np.int32, (rows,)), d_p.numpy(np.float32, (rows,))
 
 
 def accept_prefix(toks, preds, pos: int):
