@@ -28,10 +28,10 @@ FLAGS = [
     "-Wno-unused-result",
 ]
 
-# attn_prefill.hip: MFMA results in vector registers also where a kernel may use all 512 (the
+# attn_prefill.hip, tree_attn.hip: MFMA results in vector registers also where a kernel may use all 512 (the
 # default puts them in accumulation registers, and every vector instruction on the
-# prefill attention's output would move it over and back).
-FILE_FLAGS = {"attn_prefill.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"]}
+# attention's output would move it over and back).
+FILE_FLAGS = {f: ["-mllvm", "-amdgpu-mfma-vgpr-form"] for f in ("attn_prefill.hip", "tree_attn.hip")}
 
 
 def sources():

@@ -1,5 +1,17 @@
 // tree_attn.hip -- attention of every sequence's drafted tokens over a paged KV cache.
+//
+// The query heads of a kv head and a sequence's rows are its "pairs"; every K and V row serves all
+// of them.  Work is counted in units of positions over all sequences and kv heads and dealt in
+// equal runs to a fixed number of workgroups, whatever the lengths, which are read on the device;
+// a run may end inside a sequence, then its outputs, maxima and sums go to the workspace and
+// tree_attn_join_kernel adds them.
+// S^T = K . Q^T and O^T = V^T . P^T on 32x32x16 MFMA, K and V copied row by row from the pages into
+// shared memory: 32 positions x 32 pairs leave each lane with 16 scores of one pair, at just the
+// positions that the transposing LDS reads of V give the second product, so the weights never leave
+// their registers.  32-bit rows: q and the weights as two half-precision parts (2^-22), K and V
+// exact; sums, maxima and outputs in 32 bits.
 #include <algorithm>
+#include <type_traits>
 
 #include "paged.h"
 
@@ -17,97 +29,588 @@ struct TreeArgs {
     const uint64_t* mask;
     int words, width, n_seq, rows, max_rows;
     int nq, nkv, page, n_pages;
+    int page_log2;
     float scale;
     void* out;
+    int q_tiles, workers, unit;
+    float* part_o;
+    float2* part_ml;
 };
 
 __device__ inline float sigmoid(float x) { return 1.f / (1.f + expf(-x)); }
 
-// One workgroup per (row, query head); each of its 4 waves takes every fourth position with a
-// running maximum and sum, lanes over the head's dims; the waves' parts are joined at the end.
-template <class R, int HD>
-__global__ __launch_bounds__(256) void tree_attn_simple_kernel(TreeArgs p) {
+// out = acc / l (a row that saw nothing: 0), times sigmoid(gate)
+template <class T>
+__device__ inline void finish(const TreeArgs& p, int row, int head, int hd, int d, f32x4 acc, float l) {
+    f32x4 r = f32x4{0.f, 0.f, 0.f, 0.f};
+    if (l != 0.f) r = acc * (1.f / l);
+    if (p.gate) {
+        const f32x4 g = load4(static_cast<const T*>(p.gate) + row * p.g_row + head * p.g_head + d);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) r[i] *= sigmoid(g[i]);
+    }
+    store4(static_cast<T*>(p.out) + (static_cast<size_t>(row) * p.nq + head) * hd + d, r);
+}
+
+// A lane's pair (query row, query head of the kv head) and everything its tile of pairs needs.
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+typedef __attribute__((address_space(3))) void lds_void;
+typedef const __attribute__((address_space(1))) void global_void;
+
+// Positions of one round of a workgroup: a tile of 32 per wave where every wave has its own, else 64.
+constexpr int unit_of(int wp) { return wp == 1 ? 128 : 64; }
+constexpr float kRaise = 4.f;  // log2 units that a score may pass the running maximum by
+constexpr float kShift = 10.f; // weights are 2^(score - maximum + kShift): at most 2^14
+
+template <class T>
+struct Frag;
+template <>
+struct Frag<_Float16> {
+    typedef f16x8 type;
+    static __device__ f32x16 mfma(i32x4 a, i32x4 b, f32x16 c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+    }
+    static constexpr uint32_t kInf = 0x7c00u;  // exponent bits
+};
+template <>
+struct Frag<__bf16> {
+    typedef bf16x8 type;
+    static __device__ f32x16 mfma(i32x4 a, i32x4 b, f32x16 c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+    }
+    static constexpr uint32_t kInf = 0x7f80u;
+};
+
+// Units of work of every sequence: kv heads x rounds over its positions.
+__device__ inline int seq_units(const TreeArgs& p, int b, SeqSpan& s) {
+    s = seq_span(p.row_start, p.ctx_lens, b, p.rows, static_cast<int64_t>(p.width) * p.page);
+    s.n = min(s.n, p.max_rows);
+    return s.n ? (s.ctx + s.n + p.unit - 1) / p.unit : 0;
+}
+__device__ inline int64_t wave_scan64(int64_t v) {
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const int64_t x = __shfl_up(v, o, 64);
+        if (lane >= o) v += x;
+    }
+    return v;
+}
+// Sum of all units; the sequence that holds unit t, or the one that holds row `row`, and the units before it.
+struct Found {
+    int64_t total, base;
+    int b;
+};
+__device__ inline Found find_seq(const TreeArgs& p, int64_t t, int row) {
+    Found f{0, 0, -1};
+    const int lane = threadIdx.x & 63;
+    for (int b0 = 0; b0 < p.n_seq; b0 += 64) {
+        SeqSpan s{0, 0, 0};
+        int64_t u = 0;
+        if (b0 + lane < p.n_seq) u = static_cast<int64_t>(seq_units(p, b0 + lane, s)) * p.nkv;
+        const int64_t incl = wave_scan64(u);
+        const bool here = row >= 0 ? row >= s.r0 && row < s.r0 + s.n : f.total + incl > t && u > 0;
+        const unsigned long long m = __ballot(here);
+        if (f.b < 0 && m) {
+            const int l = __ffsll(m) - 1;
+            f.b = b0 + l;
+            f.base = f.total + __shfl(incl - u, l, 64);
+        }
+        f.total += __shfl(incl, 63, 64);
+    }
+    return f;
+}
+
+// The worker (of n) that has unit t of `total`: worker c has total * c / n up to total * (c + 1) / n.
+__device__ inline int64_t first_unit(int64_t total, int c, int n) { return total * c / n; }
+__device__ inline int owner(int64_t total, int64_t t, int n) {
+    int c = static_cast<int>(t * n / total);
+    while (first_unit(total, c + 1, n) <= t) ++c;
+    while (first_unit(total, c, n) > t) --c;
+    return c;
+}
+
+// Bits of the 32 positions from base on that row j of the sequence sees.
+__device__ inline uint32_t seen32(const TreeArgs& p, const SeqSpan& s, int j, int base) {
+    const int i0 = base - s.ctx;  // tree slot of the first
+    const int left = s.n - i0;    // positions that exist
+    if (left <= 0) return 0;
+    uint32_t v;
+    if (!p.mask) {
+        const int n = j - i0 + 1;
+        v = n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1;
+    } else {
+        const uint64_t* m = p.mask + static_cast<size_t>(s.r0 + j) * p.words;
+        if (i0 <= -32) {
+            v = ~0u;
+        } else if (i0 < 0) {
+            v = static_cast<uint32_t>(m[0] << -i0) | ((1u << -i0) - 1);
+        } else {
+            const int w = i0 >> 6, sh = i0 & 63;
+            uint64_t x = w < p.words ? m[w] >> sh : 0;
+            if (sh > 32 && w + 1 < p.words) x |= m[w + 1] << (64 - sh);
+            v = static_cast<uint32_t>(x);
+        }
+    }
+    return left >= 32 ? v : v & ((1u << left) - 1);
+}
+
+// One workgroup: 4 waves; WP tiles of 32 pairs (a row and one of the kv head's query heads) and
+// 4 / WP shares of the positions.  See the top of the file.
+template <class R, int HD, int WP>
+__global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void tree_attn_kernel(TreeArgs p) {
     using T = typename R::T;
     using C = typename R::C;
-    constexpr int E = HD / 64;
-    const int row = blockIdx.x, head = blockIdx.y, kv = head / (p.nq / p.nkv);
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    int b = 0;
-    SeqSpan s{};
-    for (; b < p.n_seq; ++b) {
-        s = seq_span(p.row_start, p.ctx_lens, b, p.rows, static_cast<int64_t>(p.width) * p.page);
-        if (row >= s.r0 && row < s.r0 + min(s.n, p.max_rows)) break;
-    }
-    if (b == p.n_seq) return;
-    s.n = min(s.n, p.max_rows);
-    const int j = row - s.r0;
-    float q[E], o[E];
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-        q[e] = static_cast<float>(static_cast<const T*>(p.q)[row * p.q_row + head * p.q_head + lane * E + e]);
-        o[e] = 0.f;
-    }
-    float m = -INFINITY, l = 0.f;
-    for (int pos = wave; pos < s.ctx + s.n; pos += 4) {
-        const int i = pos - s.ctx;
-        if (i >= 0) {
-            const bool sees = p.mask ? i / 64 < p.words && (p.mask[static_cast<size_t>(row) * p.words + i / 64] >> (i & 63) & 1)
-                                     : i <= j;
-            if (!sees) continue;
+    using F = Frag<C>;
+    constexpr bool kTwo = sizeof(T) == 4;  // 32-bit rows: q and the weights in two parts
+    constexpr int kUnit = unit_of(WP);
+    constexpr int WS = 4 / WP;                                // shares of the positions
+    constexpr int NT = kUnit / 32 / WS;                       // tiles of 32 positions per share and round
+    constexpr int kTiles = kUnit / 32;                        // tiles of a round
+    constexpr int U = HD / 8;                                 // 16-byte units of a row
+    constexpr int kTile = 32 * U;                             // units of a tile
+    constexpr int kPerLoad = 64 / U, kLoads = 32 / kPerLoad;  // rows of one wave load, loads of a tile
+    // WP > 1: two buffers of 64 positions; WP == 1: one of 128, a wave's tile overwritten as soon as it is used
+    __shared__ i32x4 K_s[4 * kTile], V_s[4 * kTile];
+    __shared__ float2 ml_s[4][32];
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int h = lane >> 5, col = lane & 31;
+    const int wp = wave % WP, ws = wave / WP;
+    const int G = p.nq / p.nkv;
+    // the tiles of one range of units sit on one XCD, so that its K and V come through one L2
+    const int x = blockIdx.x % 8, y = blockIdx.x / 8;
+    const int qt = y % p.q_tiles, c = y / p.q_tiles * 8 + x;
+
+    const Found all = find_seq(p, -1, -1);
+    const int64_t t0 = first_unit(all.total, c, p.workers), t1 = first_unit(all.total, c + 1, p.workers);
+    if (t0 >= t1) return;
+    Found at = find_seq(p, t0, -1);
+    int b = __builtin_amdgcn_readfirstlane(at.b);
+    int64_t base = at.base;
+
+    const int krow = col * U, kf = HD == 64 ? (col >> 1) & 7 : col & 15;
+    const int vl = lane & 15, vrow = 4 * h + (vl >> 2), vblk = (lane >> 4) & 1;
+    const float sc = p.scale * 1.44269504f;
+
+    for (int64_t t = t0; t < t1 && b < p.n_seq;) {
+        SeqSpan s;
+        const int units = seq_units(p, b, s);
+        if (units == 0) {
+            ++b;
+            continue;
         }
-        int pg = p.table[static_cast<size_t>(b) * p.width + pos / p.page];
-        if (pg < 0 || pg >= p.n_pages) pg = 0;
-        const size_t at = ((static_cast<size_t>(pg) * p.nkv + kv) * p.page + pos % p.page) * HD + lane * E;
-        const C* kr = static_cast<const C*>(p.k) + at;
-        const C* vr = static_cast<const C*>(p.v) + at;
-        float x = 0.f;
+        const int kv = static_cast<int>((t - base) / units);
+        const int ua = static_cast<int>((t - base) % units);
+        const int uz = static_cast<int>(min(static_cast<int64_t>(units), ua + (t1 - t)));
+        const bool whole = ua == 0 && uz == units;
+        const int slot = t0 < t - ua ? 1 : 0;
+        t += uz - ua;
+        const int seq = b;
+        if (t - base == static_cast<int64_t>(units) * p.nkv) {
+            base = t;
+            ++b;
+        }
+        const int pairs = s.n * G, pair0 = qt * 32 * WP;
+        if (pair0 >= pairs) continue;
+        const int mine = min(pair0 + 32 * wp + col, pairs - 1);  // this lane's pair
+        const int j = mine / G, head = kv * G + mine % G;
+        const int row = s.r0 + j;
+        // the rows' own causal limit
+        const int last = min(pair0 + 32 * WP, pairs) - 1;
+        const int L = s.ctx + (p.mask ? s.n : last / G + 1);
+        const int ub = min(uz, (L + kUnit - 1) / kUnit);
+        const int* table = p.table + static_cast<size_t>(seq) * p.width;
+
+        // row number, within the layer's cache, of position `col` of tile k of round u
+        auto entry = [&](int u, int k) {
+            const int pos = min(u * kUnit + 32 * k + col, L - 1);
+            int pg = table[pos >> p.page_log2];
+            pg = pg < 0 || pg >= p.n_pages ? 0 : pg;
+            return ((static_cast<uint32_t>(pg) * static_cast<uint32_t>(p.nkv) + kv) << p.page_log2) + (pos & (p.page - 1));
+        };
+        auto load = [&](const void* pool, i32x4* dst, uint32_t rows, bool is_v) {
 #pragma unroll
-        for (int e = 0; e < E; ++e) x += q[e] * static_cast<float>(kr[e]);
-        x = wave_sum(x) * p.scale;
-        const float mn = fmaxf(m, x);
-        const float a = m == -INFINITY ? 0.f : expf(m - mn), w = expf(x - mn);
-        m = mn;
-        l = l * a + w;
+            for (int i = 0; i < kLoads; ++i) {
+                const int r = i * kPerLoad + lane / U, u = lane % U;
+                const int f = is_v ? (HD == 64 ? (r >> 1 & 1) << 2 : (r & 3) << 2) : (HD == 64 ? r >> 1 & 7 : r & 15);
+                const uint32_t at = __shfl(rows, r, 64);
+                const char* src = static_cast<const char*>(pool) + (static_cast<size_t>(at) * U + (u ^ f)) * 16;
+                __builtin_amdgcn_global_load_lds((global_void*)src, (lds_void*)(dst + i * 64), 16, 0, 0);
+            }
+        };
+
+        // q: this lane's column of the operand, dims 16 st + 8 h ..
+        i32x4 qh[HD / 16], ql[kTwo ? HD / 16 : 1];
+        auto load_q = [&] {
+            const T* src = static_cast<const T*>(p.q) + row * p.q_row + head * p.q_head + 8 * h;
 #pragma unroll
-        for (int e = 0; e < E; ++e) o[e] = o[e] * a + w * static_cast<float>(vr[e]);
+            for (int st = 0; st < HD / 16; ++st) {
+                typename F::type hi, lo;
+#pragma unroll
+                for (int e = 0; e < 8; e += 4) {
+                    const f32x4 v = load4(src + 16 * st + e);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        hi[e + k] = static_cast<C>(v[k]);
+                        if constexpr (kTwo) lo[e + k] = static_cast<C>(v[k] - static_cast<float>(hi[e + k]));
+                    }
+                }
+                qh[st] = __builtin_bit_cast(i32x4, hi);
+                if constexpr (kTwo) ql[st] = __builtin_bit_cast(i32x4, lo);
+                // 256 dims: q lives in accumulation registers, which the MFMAs read directly
+                if constexpr (HD == 256) {
+#pragma unroll
+                    for (int d = 0; d < 4; ++d) {
+                        int a;
+                        asm("v_accvgpr_write_b32 %0, %1" : "=a"(a) : "v"(qh[st][d]));
+                        qh[st][d] = a;
+                        if constexpr (kTwo) {
+                            asm("v_accvgpr_write_b32 %0, %1" : "=a"(a) : "v"(ql[st][d]));
+                            ql[st][d] = a;
+                        }
+                    }
+                }
+            }
+        };
+        f32x16 o[HD / 32];
+#pragma unroll
+        for (int dt = 0; dt < HD / 32; ++dt)
+#pragma unroll
+            for (int v = 0; v < 16; ++v) o[dt][v] = 0.f;
+        float m = -INFINITY, l = 0.f;
+
+        // S^T = K . Q^T of a tile, in log2 units
+        auto scores = [&](const i32x4* K, f32x16& sn) {
+#pragma unroll
+            for (int v = 0; v < 16; ++v) sn[v] = 0.f;
+#pragma unroll
+            for (int st = 0; st < HD / 16; ++st) {
+                const i32x4 kk = K[krow + ((2 * st + h) ^ kf)];
+                sn = F::mfma(kk, qh[st], sn);
+                if constexpr (kTwo) sn = F::mfma(kk, ql[st], sn);
+            }
+            sn *= sc;
+        };
+        auto hide = [&](f32x16& sn, uint32_t vis) {
+#pragma unroll
+            for (int v = 0; v < 16; ++v)
+                if (!(vis >> (8 * (v >> 2) + 4 * h + (v & 3)) & 1)) sn[v] = -INFINITY;
+        };
+        // the running maximum follows the scores once one passes it by kRaise
+        auto raise = [&](f32x16 (&sn)[NT]) {
+            float mx = -INFINITY;
+#pragma unroll
+            for (int a = 0; a < NT; ++a)
+#pragma unroll
+                for (int v = 0; v < 16; ++v) mx = fmaxf(mx, sn[a][v]);
+            mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+            if (__any(mx > m + kRaise)) {
+                const float mn = fmaxf(m, mx);
+                const float alpha = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+                m = mn;
+                l *= alpha;
+#pragma unroll
+                for (int dt = 0; dt < HD / 32; ++dt) o[dt] *= alpha;
+            }
+        };
+        struct Weights {
+            i32x4 hi[2], lo[kTwo ? 2 : 1];
+        };
+        auto weights = [&](const f32x16& sn, Weights& w) {
+            const float sub = (m == -INFINITY ? 0.f : m) - kShift;
+#pragma unroll
+            for (int ks = 0; ks < 2; ++ks) {
+                typename F::type hi, lo;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const float x = __builtin_amdgcn_exp2f(sn[8 * ks + e] - sub);
+                    l += x;
+                    hi[e] = static_cast<C>(x);
+                    if constexpr (kTwo) lo[e] = static_cast<C>(x - static_cast<float>(hi[e]));
+                }
+                w.hi[ks] = __builtin_bit_cast(i32x4, hi);
+                if constexpr (kTwo) w.lo[ks] = __builtin_bit_cast(i32x4, lo);
+            }
+        };
+        // O^T += V^T . P^T of a tile; an edge tile's infinities and NaN go to the pairs that see them alone
+        auto output_of = [&]<bool edge>(std::bool_constant<edge>, const i32x4* Vt, const Weights& w, uint32_t vis) {
+            const char* V = reinterpret_cast<const char*>(Vt);
+            bool bad = false;
+#pragma unroll
+            for (int dt = 0; dt < HD / 32; ++dt)
+#pragma unroll
+                for (int ks = 0; ks < 2; ++ks) {
+                    union {
+                        s16x4 q[2];
+                        i32x4 v;
+                    } vf;
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const int r = 16 * ks + 8 * e + vrow;
+                        const int f = HD == 64 ? (r >> 1 & 1) << 2 : (r & 3) << 2;
+                        vf.q[e] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                            (lds_s16x4*)(V + (r * U + ((4 * dt + 2 * vblk + (vl >> 1 & 1)) ^ f)) * 16 + (vl & 1) * 8));
+                    }
+                    if constexpr (edge) {
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            const uint32_t z = vf.v[k];
+                            const bool lo_bad = (z & F::kInf) == F::kInf, hi_bad = (z >> 16 & F::kInf) == F::kInf;
+                            bad |= lo_bad || hi_bad;
+                            vf.v[k] = z & (lo_bad ? 0xffff0000u : ~0u) & (hi_bad ? 0xffffu : ~0u);
+                        }
+                    }
+                    o[dt] = F::mfma(vf.v, w.hi[ks], o[dt]);
+                    if constexpr (kTwo) o[dt] = F::mfma(vf.v, w.lo[ks], o[dt]);
+                }
+            if (edge && __any(bad)) {
+                const C* Ve = reinterpret_cast<const C*>(Vt);
+#pragma unroll 1
+                for (int r = 0; r < 32; ++r) {
+                    const int f = HD == 64 ? (r >> 1 & 1) << 2 : (r & 3) << 2;
+                    const bool sees = vis >> r & 1;
+#pragma unroll
+                    for (int dt = 0; dt < HD / 32; ++dt)
+#pragma unroll
+                        for (int v = 0; v < 16; ++v) {
+                            const int d = 32 * dt + 8 * (v >> 2) + 4 * h + (v & 3);
+                            const float z = static_cast<float>(Ve[r * HD + ((d >> 3) ^ f) * 8 + (d & 7)]);
+                            if (sees && !(fabsf(z) < INFINITY)) o[dt][v] += z;
+                        }
+                }
+            }
+        };
+        auto output = [&](const i32x4* Vt, const Weights& w, bool edge, uint32_t vis) {
+            if (edge)
+                output_of(std::true_type(), Vt, w, vis);
+            else
+                output_of(std::false_type(), Vt, w, vis);
+        };
+        auto round = [&](int u, f32x16 (&sn)[NT], uint32_t (&vis)[NT], bool edge) {
+            if (edge) {
+#pragma unroll
+                for (int a = 0; a < NT; ++a) {
+                    vis[a] = seen32(p, s, j, u * kUnit + 32 * (ws * NT + a));
+                    hide(sn[a], vis[a]);
+                }
+            }
+            raise(sn);
+        };
+
+        if constexpr (WP == 1) {
+            // every wave by itself: K of its next tile comes while this one's V is used, and the other way round
+            i32x4 *K = K_s + wave * kTile, *V = V_s + wave * kTile;
+            uint32_t next = 0;
+            if (ua < ub) {
+                const uint32_t rows = entry(ua, wave);
+                next = entry(min(ua + 1, ub - 1), wave);
+                load(p.k, K, rows, false);
+                load_q();
+                asm volatile("" ::: "memory");
+                load(p.v, V, rows, true);
+            }
+            for (int u = ua; u < ub; ++u) {
+                const bool edge = (u + 1) * kUnit > s.ctx, more = u + 1 < ub;
+                f32x16 sn[1];
+                uint32_t vis[1] = {~0u};
+                Weights w;
+                // all but the last kLoads loads, V's
+                asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kLoads) : "memory");
+                const uint32_t rows = next;
+                next = entry(min(u + 2, ub - 1), wave);
+                asm volatile("" ::: "memory");
+                scores(K, sn[0]);
+                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+                if (more) load(p.k, K, rows, false);
+                round(u, sn, vis, edge);
+                weights(sn[0], w);
+                // all but the next K's
+                if (more)
+                    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kLoads) : "memory");
+                else
+                    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+                output(V, w, edge, vis[0]);
+                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+                if (more) load(p.v, V, rows, true);
+            }
+        } else {
+            // wave w brings tile w % 2 of K (w < 2) or V: the next round's while this one is computed
+            const void* pool = wave < 2 ? p.k : p.v;
+            i32x4* mem = (wave < 2 ? K_s : V_s) + (wave & 1) * kTile;
+            uint32_t next = 0;
+            if (ua < ub) {
+                load(pool, mem + (ua & 1) * 2 * kTile, entry(ua, wave & 1), wave >= 2);
+                next = entry(min(ua + 1, ub - 1), wave & 1);
+            }
+            load_q();
+            for (int u = ua; u < ub; ++u) {
+                asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+                if (u + 1 < ub) {
+                    load(pool, mem + ((u + 1) & 1) * 2 * kTile, next, wave >= 2);
+                    next = entry(min(u + 2, ub - 1), wave & 1);
+                }
+                const i32x4 *K = K_s + ((u & 1) * 2 + ws * NT) * kTile, *V = V_s + ((u & 1) * 2 + ws * NT) * kTile;
+                const bool edge = (u + 1) * kUnit > s.ctx;
+                f32x16 sn[NT];
+                uint32_t vis[NT];
+                Weights w[NT];
+#pragma unroll
+                for (int a = 0; a < NT; ++a) {
+                    vis[a] = ~0u;
+                    scores(K + a * kTile, sn[a]);
+                }
+                round(u, sn, vis, edge);
+#pragma unroll
+                for (int a = 0; a < NT; ++a) weights(sn[a], w[a]);
+#pragma unroll
+                for (int a = 0; a < NT; ++a) output(V + a * kTile, w[a], edge, vis[a]);
+            }
+        }
+        l += __shfl_xor(l, 32, 64);
+
+        // ---- the waves' outputs to shared memory, [pair][HD] in 16-byte units, and out
+        __syncthreads();
+        f32x4* O_s = reinterpret_cast<f32x4*>(wave < 2 ? K_s : V_s) + (wave & 1) * (2 * kTile);
+        if (h == 0) ml_s[wave][col] = make_float2(m, l);
+#pragma unroll
+        for (int dt = 0; dt < HD / 32; ++dt)
+#pragma unroll
+            for (int v = 0; v < 16; v += 4) {
+                const int unit = 8 * dt + 2 * (v >> 2) + h;
+                O_s[col * (HD / 4) + (unit ^ (col & 15))] = f32x4{o[dt][v], o[dt][v + 1], o[dt][v + 2], o[dt][v + 3]};
+            }
+        __syncthreads();
+        constexpr int kLanes = HD / 4;
+        const int od = threadIdx.x % kLanes;
+        for (int q = threadIdx.x / kLanes; q < 32 * WP && pair0 + q < pairs; q += 256 / kLanes) {
+            const int tw = q / 32, tc = q % 32;
+            float M = -INFINITY, L2 = 0.f;
+#pragma unroll
+            for (int w = 0; w < WS; ++w) M = fmaxf(M, ml_s[w * WP + tw][tc].x);
+            f32x4 acc = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int w = 0; w < WS; ++w) {
+                const int wv = w * WP + tw;
+                const float2 ml = ml_s[wv][tc];
+                const float f = ml.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml.x - M);
+                const f32x4 part = reinterpret_cast<const f32x4*>(wv < 2 ? K_s : V_s)[(wv & 1) * (2 * kTile) + tc * kLanes + (od ^ (tc & 15))];
+                if (ml.y != 0.f) {
+                    L2 += ml.y * f;
+                    acc += part * f;
+                }
+            }
+            if (whole) {
+                finish<T>(p, s.r0 + (pair0 + q) / G, kv * G + (pair0 + q) % G, HD, 4 * od, acc, L2);
+            } else {
+                const size_t part = (static_cast<size_t>(c) * p.q_tiles + qt) * 2 + slot;
+                if (L2 != 0.f) *reinterpret_cast<f32x4*>(p.part_o + (part * (32 * WP) + q) * HD + 4 * od) = acc;
+                if (od == 0) p.part_ml[part * (32 * WP) + q] = make_float2(M, L2);
+            }
+        }
+        __syncthreads();
     }
-    __shared__ float ms[4], ls[4], os[4][HD];
-    if (lane == 0) {
-        ms[wave] = m;
-        ls[wave] = l;
+}
+
+// Joins the parts of the rows whose positions several workgroups shared.  Grid (rows, query heads).
+template <class R, int HD>
+__global__ __launch_bounds__(256) void tree_attn_join_kernel(TreeArgs p, int tile) {
+    using T = typename R::T;
+    constexpr int kLanes = HD / 4, kGroups = 256 / kLanes;
+    __shared__ f32x4 acc_s[kGroups][kLanes];
+    __shared__ float2 ml_s[kGroups];
+    const int row = blockIdx.x, head = blockIdx.y, G = p.nq / p.nkv;
+    const Found f = find_seq(p, 0, row);
+    if (f.b < 0) return;
+    SeqSpan s;
+    const int units = seq_units(p, f.b, s);
+    const int64_t t0 = f.base + static_cast<int64_t>(head / G) * units, t1 = t0 + units;
+    const int wa = owner(f.total, t0, p.workers), wz = owner(f.total, t1 - 1, p.workers);
+    if (wa == wz) return;
+    const int pair = (row - s.r0) * G + head % G, qt = pair / tile, q = pair % tile;
+    const int od = threadIdx.x % kLanes, grp = threadIdx.x / kLanes;
+    float M = -INFINITY, L = 0.f;
+    f32x4 acc = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int w = wa + grp; w <= wz; w += kGroups) {
+        if (first_unit(f.total, w, p.workers) == first_unit(f.total, w + 1, p.workers)) continue;  // has no units
+        const size_t part = ((static_cast<size_t>(w) * p.q_tiles + qt) * 2 + (first_unit(f.total, w, p.workers) < t0)) * tile + q;
+        const float2 ml = p.part_ml[part];
+        if (ml.y == 0.f) continue;
+        const f32x4 o = *reinterpret_cast<const f32x4*>(p.part_o + part * HD + 4 * od);
+        const float mn = fmaxf(M, ml.x);
+        const float fa = M == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(M - mn);
+        const float fb = ml.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml.x - mn);
+        M = mn;
+        L = L * fa + ml.y * fb;
+        acc = acc * fa + o * fb;
     }
-#pragma unroll
-    for (int e = 0; e < E; ++e) os[wave][lane * E + e] = o[e];
+    acc_s[grp][od] = acc;
+    if (od == 0) ml_s[grp] = make_float2(M, L);
     __syncthreads();
-    if (threadIdx.x >= HD) return;
-    const int d = threadIdx.x;
-    const float M = fmaxf(fmaxf(ms[0], ms[1]), fmaxf(ms[2], ms[3]));
-    float L = 0.f, O = 0.f;
-    for (int w = 0; w < 4; ++w) {
-        if (ls[w] == 0.f) continue;
-        const float f = expf(ms[w] - M);
-        L += f * ls[w];
-        O += f * os[w][d];
+    if (grp) return;
+    float mx = -INFINITY;
+#pragma unroll
+    for (int g = 0; g < kGroups; ++g) mx = fmaxf(mx, ml_s[g].x);
+    L = 0.f;
+    acc = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int g = 0; g < kGroups; ++g) {
+        if (ml_s[g].y == 0.f) continue;
+        const float fg = ml_s[g].x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml_s[g].x - mx);
+        L += ml_s[g].y * fg;
+        acc += acc_s[g][od] * fg;
     }
-    O = L == 0.f ? 0.f : O / L;
-    if (p.gate) O *= sigmoid(static_cast<float>(static_cast<const T*>(p.gate)[row * p.g_row + head * p.g_head + d]));
-    static_cast<T*>(p.out)[(static_cast<size_t>(row) * p.nq + head) * HD + d] = static_cast<T>(O);
+    finish<T>(p, row, head, HD, 4 * od, acc, L);
+}
+
+constexpr int kSlots(int hd) { return hd == 256 ? 256 : 512; }  // workgroups on the chip at once
+
+// Tiles of 32 pairs per workgroup: as many as a sequence's rows fill, the positions shared by the other waves.
+int pair_waves(int G, int max_rows) {
+    const int64_t pairs = static_cast<int64_t>(G) * max_rows;
+    return pairs <= 32 ? 1 : pairs <= 64 ? 2 : 4;
+}
+struct Split {
+    int wp, q_tiles, workers;
+};
+Split split_of(int nq, int nkv, int hd, int max_rows) {
+    Split s;
+    const int G = nq / nkv;
+    s.wp = pair_waves(G, max_rows);
+    s.q_tiles = static_cast<int>((static_cast<int64_t>(G) * max_rows + 32 * s.wp - 1) / (32 * s.wp));
+    s.workers = std::max(1, kSlots(hd) / (8 * s.q_tiles)) * 8;
+    return s;
 }
 
 size_t tree_attn_workspace_bytes(int nq, int nkv, int hd, int n_seq, int max_rows) {
-    (void)nq, (void)nkv, (void)hd, (void)n_seq, (void)max_rows;
-    return 256;
+    (void)n_seq;
+    if (nq < 1 || nkv < 1 || nq % nkv || hd < 1 || max_rows < 1) return 256;
+    const Split s = split_of(nq, nkv, hd, max_rows);
+    return static_cast<size_t>(s.workers) * s.q_tiles * 2 * 32 * s.wp * (hd * 4 + 8) + 256;
+}
+
+template <class R, int HD>
+void launch_tree(const TreeArgs& p, int wp, hipStream_t s) {
+    const dim3 grid(p.workers * p.q_tiles);
+    switch (wp) {
+    case 1: hipLaunchKernelGGL((tree_attn_kernel<R, HD, 1>), grid, dim3(256), 0, s, p); break;
+    case 2: hipLaunchKernelGGL((tree_attn_kernel<R, HD, 2>), grid, dim3(256), 0, s, p); break;
+    default: hipLaunchKernelGGL((tree_attn_kernel<R, HD, 4>), grid, dim3(256), 0, s, p); break;
+    }
+    check_launch("tree_attn_kernel");
+    hipLaunchKernelGGL((tree_attn_join_kernel<R, HD>), dim3(p.rows, p.nq), dim3(256), 0, s, p, 32 * wp);
+    check_launch("tree_attn_join_kernel");
 }
 
 template <class R>
-void launch_simple(const TreeArgs& p, int hd, hipStream_t s) {
-    const dim3 grid(p.rows, p.nq);
+void launch_tree(const TreeArgs& p, int hd, int wp, hipStream_t s) {
     switch (hd) {
-    case 64: hipLaunchKernelGGL((tree_attn_simple_kernel<R, 64>), grid, dim3(256), 0, s, p); break;
-    case 128: hipLaunchKernelGGL((tree_attn_simple_kernel<R, 128>), grid, dim3(256), 0, s, p); break;
-    default: hipLaunchKernelGGL((tree_attn_simple_kernel<R, 256>), grid, dim3(256), 0, s, p); break;
+    case 64: launch_tree<R, 64>(p, wp, s); break;
+    case 128: launch_tree<R, 128>(p, wp, s); break;
+    default: launch_tree<R, 256>(p, wp, s); break;
     }
-    check_launch("tree_attn_simple_kernel");
 }
 
 void tree_attn(const RlPagedCache* c, int layer, int dtype, const void* q, int64_t q_row, int64_t q_head, const void* gate,
@@ -127,7 +630,9 @@ void tree_attn(const RlPagedCache* c, int layer, int dtype, const void* q, int64
     RL_REQUIRE(q && table && ctx_lens && row_start && out && ws, RL_ERR_RANGE, "tree_attn: null pointer");
     check_strided(q, q_row, q_head, dtype, "tree_attn");
     if (gate) check_strided(gate, gate_row, gate_head, dtype, "tree_attn");
-    RL_REQUIRE(aligned(out, 16), RL_ERR_RANGE, "tree_attn: out must be 16-byte aligned");
+    RL_REQUIRE(aligned(out, 16) && aligned(ws, 16), RL_ERR_RANGE, "tree_attn: out and workspace must be 16-byte aligned");
+    RL_REQUIRE(static_cast<int64_t>(c->n_pages) * c->n_kv * c->page_size <= UINT32_MAX, RL_ERR_UNSUPPORTED,
+               "tree_attn: a layer's cache has more than 2^32 rows");
     RL_REQUIRE(ws_bytes >= tree_attn_workspace_bytes(nq, c->n_kv, c->head_dim, n_seq, max_rows), RL_ERR_RANGE,
                "tree_attn: workspace too small");
     TreeArgs p{};
@@ -140,12 +645,18 @@ void tree_attn(const RlPagedCache* c, int layer, int dtype, const void* q, int64
     p.n_seq = n_seq, p.rows = rows, p.max_rows = max_rows;
     p.nq = nq, p.nkv = c->n_kv, p.page = c->page_size, p.n_pages = c->n_pages;
     p.scale = scale, p.out = out;
+    while ((1 << p.page_log2) < c->page_size) ++p.page_log2;
+    const Split sp = split_of(nq, c->n_kv, c->head_dim, max_rows);
+    p.q_tiles = sp.q_tiles, p.workers = sp.workers, p.unit = unit_of(sp.wp);
+    const size_t parts = static_cast<size_t>(sp.workers) * sp.q_tiles * 2 * 32 * sp.wp;
+    p.part_o = static_cast<float*>(ws);
+    p.part_ml = reinterpret_cast<float2*>(p.part_o + parts * c->head_dim);
     if (dtype == RL_Q_F32)
-        launch_simple<RowF32>(p, c->head_dim, s);
+        launch_tree<RowF32>(p, c->head_dim, sp.wp, s);
     else if (dtype == RL_Q_F16)
-        launch_simple<RowF16>(p, c->head_dim, s);
+        launch_tree<RowF16>(p, c->head_dim, sp.wp, s);
     else
-        launch_simple<RowBF16>(p, c->head_dim, s);
+        launch_tree<RowBF16>(p, c->head_dim, sp.wp, s);
 }
 
 }  // namespace
