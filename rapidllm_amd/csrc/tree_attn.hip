@@ -83,53 +83,39 @@ struct Frag<__bf16> {
     static constexpr uint32_t kInf = 0x7f80u;
 };
 
-// Units of work of every sequence: kv heads x rounds over its positions.
-__device__ inline int seq_units(const TreeArgs& p, int b, SeqSpan& s) {
-    s = seq_span(p.row_start, p.ctx_lens, b, p.rows, static_cast<int64_t>(p.width) * p.page);
-    s.n = min(s.n, p.max_rows);
-    return s.n ? (s.ctx + s.n + p.unit - 1) / p.unit : 0;
-}
-__device__ inline int64_t wave_scan64(int64_t v) {
-    const int lane = threadIdx.x & 63;
+// The units of work of 64 sequences, one per lane: kv heads x rounds over its positions; `end` counts
+// all units up to and with the lane's.
+struct Lanes {
+    int b0;  // first sequence
+    SeqSpan s;
+    int units, end;  // per kv head; over all kv heads and sequences
+};
+__device__ inline Lanes lanes_at(const TreeArgs& p, int b0, int before) {
+    Lanes f;
+    f.b0 = b0;
+    f.s = SeqSpan{0, 0, 0};
+    const int b = b0 + (threadIdx.x & 63);
+    if (b < p.n_seq) {
+        f.s = seq_span(p.row_start, p.ctx_lens, b, p.rows, static_cast<int64_t>(p.width) * p.page);
+        f.s.n = min(f.s.n, p.max_rows);
+    }
+    f.units = f.s.n ? (f.s.ctx + f.s.n + p.unit - 1) / p.unit : 0;
+    f.end = f.units * p.nkv;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
-        const int64_t x = __shfl_up(v, o, 64);
-        if (lane >= o) v += x;
+        const int x = __shfl_up(f.end, o, 64);
+        if ((threadIdx.x & 63) >= o) f.end += x;
     }
-    return v;
-}
-// Sum of all units; the sequence that holds unit t, or the one that holds row `row`, and the units before it.
-struct Found {
-    int64_t total, base;
-    int b;
-};
-__device__ inline Found find_seq(const TreeArgs& p, int64_t t, int row) {
-    Found f{0, 0, -1};
-    const int lane = threadIdx.x & 63;
-    for (int b0 = 0; b0 < p.n_seq; b0 += 64) {
-        SeqSpan s{0, 0, 0};
-        int64_t u = 0;
-        if (b0 + lane < p.n_seq) u = static_cast<int64_t>(seq_units(p, b0 + lane, s)) * p.nkv;
-        const int64_t incl = wave_scan64(u);
-        const bool here = row >= 0 ? row >= s.r0 && row < s.r0 + s.n : f.total + incl > t && u > 0;
-        const unsigned long long m = __ballot(here);
-        if (f.b < 0 && m) {
-            const int l = __ffsll(m) - 1;
-            f.b = b0 + l;
-            f.base = f.total + __shfl(incl - u, l, 64);
-        }
-        f.total += __shfl(incl, 63, 64);
-    }
+    f.end += before;
     return f;
 }
-
-// The worker (of n) that has unit t of `total`: worker c has total * c / n up to total * (c + 1) / n.
-__device__ inline int64_t first_unit(int64_t total, int c, int n) { return total * c / n; }
-__device__ inline int owner(int64_t total, int64_t t, int n) {
-    int c = static_cast<int>(t * n / total);
-    while (first_unit(total, c + 1, n) <= t) ++c;
-    while (first_unit(total, c, n) > t) --c;
-    return c;
+__device__ inline int lane_value(int v, int lane) { return __builtin_amdgcn_readlane(v, lane); }
+// Units of a workgroup: workgroup c has units c * per up to (c + 1) * per of the first 64 sequences' f and
+// the rest.
+__device__ inline int total_units(const TreeArgs& p, const Lanes& f) {
+    int total = lane_value(f.end, 63);
+    for (int b0 = 64; b0 < p.n_seq; b0 += 64) total = lane_value(lanes_at(p, b0, total).end, 63);
+    return total;
 }
 
 // Bits of the 32 positions from base on that row j of the sequence sees.
@@ -155,6 +141,20 @@ __device__ inline uint32_t seen32(const TreeArgs& p, const SeqSpan& s, int j, in
         }
     }
     return left >= 32 ? v : v & ((1u << left) - 1);
+}
+
+template <int HD>
+__device__ inline int k_swap(int r) {
+    return HD == 64 ? r >> 1 & 7 : r & 15;
+}
+template <int HD>
+__device__ inline int v_swap(int r) {
+    return HD == 64 ? (r >> 1 & 1) << 2 : (r & 3) << 2;
+}
+// the same value, of which the compiler knows nothing
+__device__ inline int opaque(int v) {
+    asm volatile("" : "+v"(v));
+    return v;
 }
 
 // One workgroup: 4 waves; WP tiles of 32 pairs (a row and one of the kv head's query heads) and
@@ -184,35 +184,31 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void tree_attn_kernel(TreeA
     const int x = blockIdx.x % 8, y = blockIdx.x / 8;
     const int qt = y % p.q_tiles, c = y / p.q_tiles * 8 + x;
 
-    const Found all = find_seq(p, -1, -1);
-    const int64_t t0 = first_unit(all.total, c, p.workers), t1 = first_unit(all.total, c + 1, p.workers);
+    Lanes f = lanes_at(p, 0, 0);
+    const int total = total_units(p, f);
+    const int per = (total + p.workers - 1) / p.workers;
+    const int t0 = min(c * per, total), t1 = min(t0 + per, total);
     if (t0 >= t1) return;
-    Found at = find_seq(p, t0, -1);
-    int b = __builtin_amdgcn_readfirstlane(at.b);
-    int64_t base = at.base;
 
-    const int krow = col * U, kf = HD == 64 ? (col >> 1) & 7 : col & 15;
-    const int vl = lane & 15, vrow = 4 * h + (vl >> 2), vblk = (lane >> 4) & 1;
+    // Shared-memory addresses (bytes) are a lane's own part, xor a constant: unit u of K row r sits at
+    // u ^ (r & 15), of V row r at u ^ 4 (r & 3), so that neither reads nor rows share banks (64 dims, two
+    // rows in 256 bytes: by r / 2).  Kept opaque below: a register each for every constant is too many.
+    const int vl = lane & 15, vrow = 4 * h + (vl >> 2);
+    const int kaddr = (col * U + (h ^ k_swap<HD>(col))) * 16;
+    const int vaddr = (vrow * U + (v_swap<HD>(vrow) | ((lane >> 4) & 1) * 2 | (vl >> 1 & 1))) * 16 + (vl & 1) * 8;
     const float sc = p.scale * 1.44269504f;
 
-    for (int64_t t = t0; t < t1 && b < p.n_seq;) {
-        SeqSpan s;
-        const int units = seq_units(p, b, s);
-        if (units == 0) {
-            ++b;
-            continue;
-        }
-        const int kv = static_cast<int>((t - base) / units);
-        const int ua = static_cast<int>((t - base) % units);
-        const int uz = static_cast<int>(min(static_cast<int64_t>(units), ua + (t1 - t)));
+    for (int t = t0; t < t1;) {
+        unsigned long long after;
+        while (!(after = __ballot(f.end > t)) && f.b0 + 64 < p.n_seq) f = lanes_at(p, f.b0 + 64, lane_value(f.end, 63));
+        if (!after) break;
+        const int fl = __ffsll(after) - 1, seq = f.b0 + fl;
+        const SeqSpan s{lane_value(f.s.r0, fl), lane_value(f.s.n, fl), lane_value(f.s.ctx, fl)};
+        const int units = lane_value(f.units, fl), at = t - (lane_value(f.end, fl) - units * p.nkv);
+        const int kv = at / units, ua = at % units, uz = min(units, ua + (t1 - t));
         const bool whole = ua == 0 && uz == units;
         const int slot = t0 < t - ua ? 1 : 0;
         t += uz - ua;
-        const int seq = b;
-        if (t - base == static_cast<int64_t>(units) * p.nkv) {
-            base = t;
-            ++b;
-        }
         const int pairs = s.n * G, pair0 = qt * 32 * WP;
         if (pair0 >= pairs) continue;
         const int mine = min(pair0 + 32 * wp + col, pairs - 1);  // this lane's pair
@@ -232,10 +228,12 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void tree_attn_kernel(TreeA
             return ((static_cast<uint32_t>(pg) * static_cast<uint32_t>(p.nkv) + kv) << p.page_log2) + (pos & (p.page - 1));
         };
         auto load = [&](const void* pool, i32x4* dst, uint32_t rows, bool is_v) {
+            const int own = opaque(lane);
+            rows = opaque(rows);
 #pragma unroll
             for (int i = 0; i < kLoads; ++i) {
-                const int r = i * kPerLoad + lane / U, u = lane % U;
-                const int f = is_v ? (HD == 64 ? (r >> 1 & 1) << 2 : (r & 3) << 2) : (HD == 64 ? r >> 1 & 7 : r & 15);
+                const int r = i * kPerLoad + own / U, u = own % U;
+                const int f = is_v ? v_swap<HD>(r) : k_swap<HD>(r);
                 const uint32_t at = __shfl(rows, r, 64);
                 const char* src = static_cast<const char*>(pool) + (static_cast<size_t>(at) * U + (u ^ f)) * 16;
                 __builtin_amdgcn_global_load_lds((global_void*)src, (lds_void*)(dst + i * 64), 16, 0, 0);
@@ -283,12 +281,14 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void tree_attn_kernel(TreeA
         float m = -INFINITY, l = 0.f;
 
         // S^T = K . Q^T of a tile, in log2 units
-        auto scores = [&](const i32x4* K, f32x16& sn) {
+        auto scores = [&](const i32x4* Kt, f32x16& sn) {
+            const char* K = reinterpret_cast<const char*>(Kt);
+            const int own = opaque(kaddr);
 #pragma unroll
             for (int v = 0; v < 16; ++v) sn[v] = 0.f;
 #pragma unroll
             for (int st = 0; st < HD / 16; ++st) {
-                const i32x4 kk = K[krow + ((2 * st + h) ^ kf)];
+                const i32x4 kk = *reinterpret_cast<const i32x4*>(K + (own ^ 32 * st));
                 sn = F::mfma(kk, qh[st], sn);
                 if constexpr (kTwo) sn = F::mfma(kk, ql[st], sn);
             }
@@ -336,8 +336,9 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void tree_attn_kernel(TreeA
             }
         };
         // O^T += V^T . P^T of a tile; an edge tile's infinities and NaN go to the pairs that see them alone
-        auto output_of = [&]<bool edge>(std::bool_constant<edge>, const i32x4* Vt, const Weights& w, uint32_t vis) {
+        auto output = [&]<bool edge>(std::bool_constant<edge>, const i32x4* Vt, const Weights& w, uint32_t vis) {
             const char* V = reinterpret_cast<const char*>(Vt);
+            const int own = opaque(vaddr);
             bool bad = false;
 #pragma unroll
             for (int dt = 0; dt < HD / 32; ++dt)
@@ -348,12 +349,9 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void tree_attn_kernel(TreeA
                         i32x4 v;
                     } vf;
 #pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        const int r = 16 * ks + 8 * e + vrow;
-                        const int f = HD == 64 ? (r >> 1 & 1) << 2 : (r & 3) << 2;
+                    for (int e = 0; e < 2; ++e)
                         vf.q[e] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                            (lds_s16x4*)(V + (r * U + ((4 * dt + 2 * vblk + (vl >> 1 & 1)) ^ f)) * 16 + (vl & 1) * 8));
-                    }
+                            (lds_s16x4*)(V + (own ^ 64 * dt) + (16 * ks + 8 * e) * U * 16));
                     if constexpr (edge) {
 #pragma unroll
                         for (int k = 0; k < 4; ++k) {
@@ -370,36 +368,21 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void tree_attn_kernel(TreeA
                 const C* Ve = reinterpret_cast<const C*>(Vt);
 #pragma unroll 1
                 for (int r = 0; r < 32; ++r) {
-                    const int f = HD == 64 ? (r >> 1 & 1) << 2 : (r & 3) << 2;
                     const bool sees = vis >> r & 1;
 #pragma unroll
                     for (int dt = 0; dt < HD / 32; ++dt)
 #pragma unroll
                         for (int v = 0; v < 16; ++v) {
                             const int d = 32 * dt + 8 * (v >> 2) + 4 * h + (v & 3);
-                            const float z = static_cast<float>(Ve[r * HD + ((d >> 3) ^ f) * 8 + (d & 7)]);
+                            const float z = static_cast<float>(Ve[r * HD + ((d >> 3) ^ v_swap<HD>(r)) * 8 + (d & 7)]);
                             if (sees && !(fabsf(z) < INFINITY)) o[dt][v] += z;
+                            if (v % 4 == 3) asm volatile("" ::: "memory");
                         }
                 }
             }
         };
-        auto output = [&](const i32x4* Vt, const Weights& w, bool edge, uint32_t vis) {
-            if (edge)
-                output_of(std::true_type(), Vt, w, vis);
-            else
-                output_of(std::false_type(), Vt, w, vis);
-        };
-        auto round = [&](int u, f32x16 (&sn)[NT], uint32_t (&vis)[NT], bool edge) {
-            if (edge) {
-#pragma unroll
-                for (int a = 0; a < NT; ++a) {
-                    vis[a] = seen32(p, s, j, u * kUnit + 32 * (ws * NT + a));
-                    hide(sn[a], vis[a]);
-                }
-            }
-            raise(sn);
-        };
-
+        // rounds up to u_edge hold positions of the context alone
+        const int u_edge = min(max(s.ctx / kUnit, ua), ub);
         if constexpr (WP == 1) {
             // every wave by itself: K of its next tile comes while this one's V is used, and the other way round
             i32x4 *K = K_s + wave * kTile, *V = V_s + wave * kTile;
@@ -412,30 +395,35 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void tree_attn_kernel(TreeA
                 asm volatile("" ::: "memory");
                 load(p.v, V, rows, true);
             }
-            for (int u = ua; u < ub; ++u) {
-                const bool edge = (u + 1) * kUnit > s.ctx, more = u + 1 < ub;
-                f32x16 sn[1];
-                uint32_t vis[1] = {~0u};
-                Weights w;
-                // all but the last kLoads loads, V's
-                asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kLoads) : "memory");
-                const uint32_t rows = next;
-                next = entry(min(u + 2, ub - 1), wave);
-                asm volatile("" ::: "memory");
-                scores(K, sn[0]);
-                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-                if (more) load(p.k, K, rows, false);
-                round(u, sn, vis, edge);
-                weights(sn[0], w);
-                // all but the next K's
-                if (more)
+            auto rounds = [&]<bool edge>(std::bool_constant<edge> e, int from, int to) {
+                for (int u = from; u < to; ++u) {
+                    const bool more = u + 1 < ub;
+                    f32x16 sn[1];
+                    uint32_t vis = ~0u;
+                    Weights w;
+                    // all but the last kLoads loads, V's
                     asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kLoads) : "memory");
-                else
-                    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-                output(V, w, edge, vis[0]);
-                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-                if (more) load(p.v, V, rows, true);
-            }
+                    const uint32_t rows = next;
+                    next = entry(min(u + 2, ub - 1), wave);
+                    asm volatile("" ::: "memory");
+                    scores(K, sn[0]);
+                    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+                    if (more) load(p.k, K, rows, false);
+                    if constexpr (edge) hide(sn[0], vis = seen32(p, s, j, u * kUnit + 32 * wave));
+                    raise(sn);
+                    weights(sn[0], w);
+                    // all but the next K's
+                    if (more)
+                        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kLoads) : "memory");
+                    else
+                        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+                    output(e, V, w, vis);
+                    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+                    if (more) load(p.v, V, rows, true);
+                }
+            };
+            rounds(std::false_type(), ua, u_edge);
+            rounds(std::true_type(), u_edge, ub);
         } else {
             // wave w brings tile w % 2 of K (w < 2) or V: the next round's while this one is computed
             const void* pool = wave < 2 ? p.k : p.v;
@@ -446,42 +434,46 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void tree_attn_kernel(TreeA
                 next = entry(min(ua + 1, ub - 1), wave & 1);
             }
             load_q();
-            for (int u = ua; u < ub; ++u) {
-                asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-                if (u + 1 < ub) {
-                    load(pool, mem + ((u + 1) & 1) * 2 * kTile, next, wave >= 2);
-                    next = entry(min(u + 2, ub - 1), wave & 1);
+            auto rounds = [&]<bool edge>(std::bool_constant<edge> e, int from, int to) {
+                for (int u = from; u < to; ++u) {
+                    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+                    if (u + 1 < ub) {
+                        load(pool, mem + ((u + 1) & 1) * 2 * kTile, next, wave >= 2);
+                        next = entry(min(u + 2, ub - 1), wave & 1);
+                    }
+                    const i32x4 *K = K_s + ((u & 1) * 2 + ws * NT) * kTile, *V = V_s + ((u & 1) * 2 + ws * NT) * kTile;
+                    f32x16 sn[NT];
+                    uint32_t vis[NT];
+                    Weights w[NT];
+#pragma unroll
+                    for (int a = 0; a < NT; ++a) {
+                        scores(K + a * kTile, sn[a]);
+                        vis[a] = ~0u;
+                        if constexpr (edge) hide(sn[a], vis[a] = seen32(p, s, j, u * kUnit + 32 * (ws * NT + a)));
+                    }
+                    raise(sn);
+#pragma unroll
+                    for (int a = 0; a < NT; ++a) weights(sn[a], w[a]);
+#pragma unroll
+                    for (int a = 0; a < NT; ++a) output(e, V + a * kTile, w[a], vis[a]);
                 }
-                const i32x4 *K = K_s + ((u & 1) * 2 + ws * NT) * kTile, *V = V_s + ((u & 1) * 2 + ws * NT) * kTile;
-                const bool edge = (u + 1) * kUnit > s.ctx;
-                f32x16 sn[NT];
-                uint32_t vis[NT];
-                Weights w[NT];
-#pragma unroll
-                for (int a = 0; a < NT; ++a) {
-                    vis[a] = ~0u;
-                    scores(K + a * kTile, sn[a]);
-                }
-                round(u, sn, vis, edge);
-#pragma unroll
-                for (int a = 0; a < NT; ++a) weights(sn[a], w[a]);
-#pragma unroll
-                for (int a = 0; a < NT; ++a) output(V + a * kTile, w[a], edge, vis[a]);
-            }
+            };
+            rounds(std::false_type(), ua, u_edge);
+            rounds(std::true_type(), u_edge, ub);
         }
         l += __shfl_xor(l, 32, 64);
 
         // ---- the waves' outputs to shared memory, [pair][HD] in 16-byte units, and out
         __syncthreads();
-        f32x4* O_s = reinterpret_cast<f32x4*>(wave < 2 ? K_s : V_s) + (wave & 1) * (2 * kTile);
+        char* O_s = reinterpret_cast<char*>((wave < 2 ? K_s : V_s) + (wave & 1) * (2 * kTile));
+        const int oaddr = opaque((col * (HD / 4) + (h ^ (col & 15))) * 16);
         if (h == 0) ml_s[wave][col] = make_float2(m, l);
 #pragma unroll
         for (int dt = 0; dt < HD / 32; ++dt)
 #pragma unroll
-            for (int v = 0; v < 16; v += 4) {
-                const int unit = 8 * dt + 2 * (v >> 2) + h;
-                O_s[col * (HD / 4) + (unit ^ (col & 15))] = f32x4{o[dt][v], o[dt][v + 1], o[dt][v + 2], o[dt][v + 3]};
-            }
+            for (int v = 0; v < 16; v += 4)
+                *reinterpret_cast<f32x4*>(O_s + (oaddr ^ (8 * dt + 2 * (v >> 2)) * 16)) =
+                    f32x4{o[dt][v], o[dt][v + 1], o[dt][v + 2], o[dt][v + 3]};
         __syncthreads();
         constexpr int kLanes = HD / 4;
         const int od = threadIdx.x % kLanes;
@@ -514,55 +506,66 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void tree_attn_kernel(TreeA
     }
 }
 
-// Joins the parts of the rows whose positions several workgroups shared.  Grid (rows, query heads).
-template <class R, int HD>
+// Joins the parts of the rows whose positions several workgroups shared.  kWaves waves per (row, query
+// head): 4 where there are few of them, each a share of the parts, else 1.
+template <class R, int HD, int kWaves>
 __global__ __launch_bounds__(256) void tree_attn_join_kernel(TreeArgs p, int tile) {
     using T = typename R::T;
-    constexpr int kLanes = HD / 4, kGroups = 256 / kLanes;
-    __shared__ f32x4 acc_s[kGroups][kLanes];
-    __shared__ float2 ml_s[kGroups];
-    const int row = blockIdx.x, head = blockIdx.y, G = p.nq / p.nkv;
-    const Found f = find_seq(p, 0, row);
-    if (f.b < 0) return;
-    SeqSpan s;
-    const int units = seq_units(p, f.b, s);
-    const int64_t t0 = f.base + static_cast<int64_t>(head / G) * units, t1 = t0 + units;
-    const int wa = owner(f.total, t0, p.workers), wz = owner(f.total, t1 - 1, p.workers);
-    if (wa == wz) return;
-    const int pair = (row - s.r0) * G + head % G, qt = pair / tile, q = pair % tile;
-    const int od = threadIdx.x % kLanes, grp = threadIdx.x / kLanes;
+    constexpr int kLanes = HD / 4, kGroups = kWaves * 64 / kLanes;  // lanes of an output, parts side by side
+    constexpr int kSets = 4 / kWaves;
+    __shared__ f32x4 acc_s[kSets][kGroups][kLanes];
+    const int lane = threadIdx.x & 63, set = threadIdx.x / (64 * kWaves);
+    const int item = blockIdx.x * kSets + set, row = item / p.nq, head = item % p.nq, G = p.nq / p.nkv;
+    Lanes f = lanes_at(p, 0, 0);
+    const int total = total_units(p, f);
+    const int per = (total + p.workers - 1) / p.workers;
+    unsigned long long m;
+    while (!(m = __ballot(row >= f.s.r0 && row < f.s.r0 + f.s.n)) && f.b0 + 64 < p.n_seq)
+        f = lanes_at(p, f.b0 + 64, lane_value(f.end, 63));
+    int wa = 0, wz = 0, q = 0, qt = 0, t0 = 0;
+    if (m && row < p.rows) {
+        const int fl = __ffsll(m) - 1, units = lane_value(f.units, fl);
+        t0 = lane_value(f.end, fl) - units * p.nkv + head / G * units;
+        wa = t0 / per, wz = (t0 + units - 1) / per;
+        const int pair = (row - lane_value(f.s.r0, fl)) * G + head % G;
+        qt = pair / tile, q = pair % tile;
+    }
+    const int od = threadIdx.x % kLanes, grp = threadIdx.x % (64 * kWaves) / kLanes;
     float M = -INFINITY, L = 0.f;
     f32x4 acc = f32x4{0.f, 0.f, 0.f, 0.f};
-    for (int w = wa + grp; w <= wz; w += kGroups) {
-        if (first_unit(f.total, w, p.workers) == first_unit(f.total, w + 1, p.workers)) continue;  // has no units
-        const size_t part = ((static_cast<size_t>(w) * p.q_tiles + qt) * 2 + (first_unit(f.total, w, p.workers) < t0)) * tile + q;
-        const float2 ml = p.part_ml[part];
-        if (ml.y == 0.f) continue;
-        const f32x4 o = *reinterpret_cast<const f32x4*>(p.part_o + part * HD + 4 * od);
-        const float mn = fmaxf(M, ml.x);
-        const float fa = M == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(M - mn);
-        const float fb = ml.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml.x - mn);
-        M = mn;
-        L = L * fa + ml.y * fb;
-        acc = acc * fa + o * fb;
+    if (wa != wz) {
+        for (int w0 = wa; w0 <= wz; w0 += 64) {
+            // the parts' weights, one per lane, then their outputs
+            const int w = w0 + lane;
+            const size_t part = ((static_cast<size_t>(min(w, wz)) * p.q_tiles + qt) * 2 + (min(w, wz) * per < t0)) * tile + q;
+            const float2 ml = p.part_ml[part];
+            const float mine = w <= wz && ml.y != 0.f ? ml.x : -INFINITY;
+            const float mn = fmaxf(M, wave_max(mine));
+            const float old = M == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(M - mn);
+            const float wt = mine == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mine - mn);
+            const float lw = w <= wz && ml.y != 0.f ? ml.y * wt : 0.f;
+            M = mn;
+            L = L * old + wave_sum(lw);
+            acc = acc * old;
+            const int n = min(64, wz - w0 + 1);
+#pragma unroll 4
+            for (int i = grp; i < n; i += kGroups) {
+                const float fw = __shfl(wt, i, 64);
+                const size_t at = ((static_cast<size_t>(w0 + i) * p.q_tiles + qt) * 2 + ((w0 + i) * per < t0)) * tile + q;
+                const f32x4 o = *reinterpret_cast<const f32x4*>(p.part_o + at * HD + 4 * od);
+                if (fw != 0.f) acc += o * fw;
+            }
+        }
     }
-    acc_s[grp][od] = acc;
-    if (od == 0) ml_s[grp] = make_float2(M, L);
-    __syncthreads();
-    if (grp) return;
-    float mx = -INFINITY;
+    if constexpr (kGroups > 1) {
+        acc_s[set][grp][od] = acc;
+        __syncthreads();
+        if (grp == 0) {
 #pragma unroll
-    for (int g = 0; g < kGroups; ++g) mx = fmaxf(mx, ml_s[g].x);
-    L = 0.f;
-    acc = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int g = 0; g < kGroups; ++g) {
-        if (ml_s[g].y == 0.f) continue;
-        const float fg = ml_s[g].x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml_s[g].x - mx);
-        L += ml_s[g].y * fg;
-        acc += acc_s[g][od] * fg;
+            for (int g = 1; g < kGroups; ++g) acc += acc_s[set][g][od];
+        }
     }
-    finish<T>(p, row, head, HD, 4 * od, acc, L);
+    if (wa != wz && grp == 0) finish<T>(p, row, head, HD, 4 * od, acc, L);
 }
 
 constexpr int kSlots(int hd) { return hd == 256 ? 256 : 512; }  // workgroups on the chip at once
@@ -600,7 +603,12 @@ void launch_tree(const TreeArgs& p, int wp, hipStream_t s) {
     default: hipLaunchKernelGGL((tree_attn_kernel<R, HD, 4>), grid, dim3(256), 0, s, p); break;
     }
     check_launch("tree_attn_kernel");
-    hipLaunchKernelGGL((tree_attn_join_kernel<R, HD>), dim3(p.rows, p.nq), dim3(256), 0, s, p, 32 * wp);
+    // 4096 outputs: a wave each
+    const int64_t outs = static_cast<int64_t>(p.rows) * p.nq;
+    if (outs < 4096)
+        hipLaunchKernelGGL((tree_attn_join_kernel<R, HD, 4>), dim3(outs), dim3(256), 0, s, p, 32 * wp);
+    else
+        hipLaunchKernelGGL((tree_attn_join_kernel<R, HD, 1>), dim3((outs + 3) / 4), dim3(256), 0, s, p, 32 * wp);
     check_launch("tree_attn_join_kernel");
 }
 
@@ -631,6 +639,9 @@ void tree_attn(const RlPagedCache* c, int layer, int dtype, const void* q, int64
     check_strided(q, q_row, q_head, dtype, "tree_attn");
     if (gate) check_strided(gate, gate_row, gate_head, dtype, "tree_attn");
     RL_REQUIRE(aligned(out, 16) && aligned(ws, 16), RL_ERR_RANGE, "tree_attn: out and workspace must be 16-byte aligned");
+    RL_REQUIRE(static_cast<double>(n_seq) * c->n_kv * (static_cast<double>(width) * c->page_size / 64 + 1) < INT32_MAX &&
+                   static_cast<int64_t>(rows) * nq < INT32_MAX,
+               RL_ERR_UNSUPPORTED, "tree_attn: more than 2^31 units of work");
     RL_REQUIRE(static_cast<int64_t>(c->n_pages) * c->n_kv * c->page_size <= UINT32_MAX, RL_ERR_UNSUPPORTED,
                "tree_attn: a layer's cache has more than 2^32 rows");
     RL_REQUIRE(ws_bytes >= tree_attn_workspace_bytes(nq, c->n_kv, c->head_dim, n_seq, max_rows), RL_ERR_RANGE,
