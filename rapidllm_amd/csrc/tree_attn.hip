@@ -61,6 +61,7 @@ typedef const __attribute__((address_space(1))) void global_void;
 
 // Positions of one round of a workgroup: a tile of 32 per wave where every wave has its own, else 64.
 constexpr int unit_of(int wp) { return wp == 1 ? 128 : 64; }
+constexpr int kAhead = 4;        // operands read from shared memory ahead of their products
 constexpr float kRaise = 4.f;  // log2 units that a score may pass the running maximum by
 constexpr float kShift = 10.f; // weights are 2^(score - maximum + kShift): at most 2^14
 
@@ -157,6 +158,9 @@ __device__ inline int opaque(int v) {
     return v;
 }
 
+// Keeps a product where it stands among the reads and the vector work (the compiler sinks it to its use).
+__device__ inline void pin(f32x16& v) { asm volatile("" : "+v"(v)); }
+
 // One workgroup: 4 waves; WP tiles of 32 pairs (a row and one of the kv head's query heads) and
 // 4 / WP shares of the positions.  See the top of the file.
 template <class R, int HD, int WP>
@@ -220,25 +224,47 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void tree_attn_kernel(TreeA
         const int ub = min(uz, (L + kUnit - 1) / kUnit);
         const int* table = p.table + static_cast<size_t>(seq) * p.width;
 
-        // row number, within the layer's cache, of position `col` of tile k of round u
-        auto entry = [&](int u, int k) {
-            const int pos = min(u * kUnit + 32 * k + col, L - 1);
-            int pg = table[pos >> p.page_log2];
+        // The page of position `col` of tile k of round u as the table has it, and the position's row number
+        // within the layer's cache.  (Apart: the load is in flight for a round.)
+        auto page_of = [&](int u, int k) { return table[min(u * kUnit + 32 * k + col, L - 1) >> p.page_log2]; };
+        auto row_of = [&](int pg, int u, int k) {
             pg = pg < 0 || pg >= p.n_pages ? 0 : pg;
-            return ((static_cast<uint32_t>(pg) * static_cast<uint32_t>(p.nkv) + kv) << p.page_log2) + (pos & (p.page - 1));
+            return ((static_cast<uint32_t>(pg) * static_cast<uint32_t>(p.nkv) + kv) << p.page_log2) +
+                   (min(u * kUnit + 32 * k + col, L - 1) & (p.page - 1));
         };
-        auto load = [&](const void* pool, i32x4* dst, uint32_t rows, bool is_v) {
-            const int own = opaque(lane);
-            rows = opaque(rows);
-#pragma unroll
-            for (int i = 0; i < kLoads; ++i) {
-                const int r = i * kPerLoad + own / U, u = own % U;
+        // Load i of a tile: kPerLoad rows.  Where they lie in one page (`runs`), their address is a scalar and
+        // a lane's offset; else, and for rows past the last position, each row's own.
+        auto load1 = [&](const void* pool, i32x4* dst, uint32_t rows, bool is_v, bool runs, int own, int i) {
+            const char* src;
+            if (runs) {
+                const int f = is_v ? v_swap<HD>(i * kPerLoad) : k_swap<HD>(i * kPerLoad);
+                const uint32_t r0 = __builtin_amdgcn_readlane(rows, i * kPerLoad);
+                src = static_cast<const char*>(pool) + static_cast<size_t>(r0) * (U * 16) + static_cast<uint32_t>(own ^ f * 16);
+            } else {
+                const int r = i * kPerLoad + own / (U * 16), u = lane % U;
                 const int f = is_v ? v_swap<HD>(r) : k_swap<HD>(r);
                 const uint32_t at = __shfl(rows, r, 64);
-                const char* src = static_cast<const char*>(pool) + (static_cast<size_t>(at) * U + (u ^ f)) * 16;
-                __builtin_amdgcn_global_load_lds((global_void*)src, (lds_void*)(dst + i * 64), 16, 0, 0);
+                src = static_cast<const char*>(pool) + (static_cast<size_t>(at) * U + (u ^ f)) * 16;
+            }
+            __builtin_amdgcn_global_load_lds((global_void*)src, (lds_void*)(dst + i * 64), 16, 0, 0);
+        };
+        // a lane's offset within a load's rows: the swaps of rows i * kPerLoad + lane / U are those of the two parts, xor
+        auto own_offset = [&](bool is_v) {
+            const int r = lane / U, f = is_v ? v_swap<HD>(r) : k_swap<HD>(r);
+            return opaque(r * U * 16 + ((lane % U) ^ f) * 16);
+        };
+        auto load = [&](const void* pool, i32x4* dst, uint32_t rows, bool is_v, bool runs) {
+            const int own = own_offset(is_v);
+            rows = opaque(rows);
+            if (runs) {
+#pragma unroll
+                for (int i = 0; i < kLoads; ++i) load1(pool, dst, rows, is_v, true, own, i);
+            } else {
+#pragma unroll
+                for (int i = 0; i < kLoads; ++i) load1(pool, dst, rows, is_v, false, own, i);
             }
         };
+        const bool page_runs = p.page >= kPerLoad;
 
         // q: this lane's column of the operand, dims 16 st + 8 h ..
         i32x4 qh[HD / 16], ql[kTwo ? HD / 16 : 1];
@@ -280,19 +306,30 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void tree_attn_kernel(TreeA
             for (int v = 0; v < 16; ++v) o[dt][v] = 0.f;
         float m = -INFINITY, l = 0.f;
 
-        // S^T = K . Q^T of a tile, in log2 units
-        auto scores = [&](const i32x4* Kt, f32x16& sn) {
+        // S^T = K . Q^T of the tiles, in log2 units
+        auto scores = [&](const i32x4* Kt, f32x16 (&sn)[NT]) {
             const char* K = reinterpret_cast<const char*>(Kt);
             const int own = opaque(kaddr);
 #pragma unroll
-            for (int v = 0; v < 16; ++v) sn[v] = 0.f;
+            for (int a = 0; a < NT; ++a)
 #pragma unroll
-            for (int st = 0; st < HD / 16; ++st) {
-                const i32x4 kk = *reinterpret_cast<const i32x4*>(K + (own ^ 32 * st));
-                sn = F::mfma(kk, qh[st], sn);
-                if constexpr (kTwo) sn = F::mfma(kk, ql[st], sn);
+                for (int v = 0; v < 16; ++v) sn[a][v] = 0.f;
+            // product i: dims 16 (i / NT), tile i % NT; its K read kAhead products before
+            constexpr int N = NT * HD / 16;
+            auto read = [&](int i) { return *reinterpret_cast<const i32x4*>(K + (own ^ 32 * (i / NT)) + (i % NT) * kTile * 16); };
+            i32x4 kk[kAhead];
+#pragma unroll
+            for (int i = 0; i < kAhead; ++i) kk[i] = read(i);
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                sn[i % NT] = F::mfma(kk[i % kAhead], qh[i / NT], sn[i % NT]);
+                if constexpr (kTwo) sn[i % NT] = F::mfma(kk[i % kAhead], ql[i / NT], sn[i % NT]);
+                pin(sn[i % NT]);
+                if (i + kAhead < N) kk[i % kAhead] = read(i + kAhead);
+                __builtin_amdgcn_sched_barrier(0);
             }
-            sn *= sc;
+#pragma unroll
+            for (int a = 0; a < NT; ++a) sn[a] *= sc;
         };
         auto hide = [&](f32x16& sn, uint32_t vis) {
 #pragma unroll
@@ -317,53 +354,64 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void tree_attn_kernel(TreeA
             }
         };
         struct Weights {
-            i32x4 hi[2], lo[kTwo ? 2 : 1];
+            typename F::type hi[2], lo[kTwo ? 2 : 1];
         };
-        auto weights = [&](const f32x16& sn, Weights& w) {
-            const float sub = (m == -INFINITY ? 0.f : m) - kShift;
+        // weights 2 i and 2 i + 1 of a tile
+        auto weights2 = [&](const f32x16& sn, Weights& w, float sub, int i) {
 #pragma unroll
-            for (int ks = 0; ks < 2; ++ks) {
-                typename F::type hi, lo;
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const float x = __builtin_amdgcn_exp2f(sn[8 * ks + e] - sub);
-                    l += x;
-                    hi[e] = static_cast<C>(x);
-                    if constexpr (kTwo) lo[e] = static_cast<C>(x - static_cast<float>(hi[e]));
-                }
-                w.hi[ks] = __builtin_bit_cast(i32x4, hi);
-                if constexpr (kTwo) w.lo[ks] = __builtin_bit_cast(i32x4, lo);
+            for (int e = 2 * i; e < 2 * i + 2; ++e) {
+                const float x = __builtin_amdgcn_exp2f(sn[e] - sub);
+                l += x;
+                const C hi = static_cast<C>(x);
+                w.hi[e >> 3][e & 7] = hi;
+                if constexpr (kTwo) w.lo[e >> 3][e & 7] = static_cast<C>(x - static_cast<float>(hi));
             }
         };
-        // O^T += V^T . P^T of a tile; an edge tile's infinities and NaN go to the pairs that see them alone
-        auto output = [&]<bool edge>(std::bool_constant<edge>, const i32x4* Vt, const Weights& w, uint32_t vis) {
+        auto weights = [&](const f32x16& sn, Weights& w, float sub) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) weights2(sn, w, sub, i);
+        };
+        auto level = [&] { return (m == -INFINITY ? 0.f : m) - kShift; };
+        // O^T += V^T . P^T of a tile; an edge tile's infinities and NaN go to the pairs that see them alone.
+        // side(i): what is computed under product i
+        auto output = [&]<bool edge>(std::bool_constant<edge>, const i32x4* Vt, const Weights& w, uint32_t vis, auto side) {
             const char* V = reinterpret_cast<const char*>(Vt);
             const int own = opaque(vaddr);
             bool bad = false;
+            constexpr int N = HD / 16;  // product i: dims 32 (i / 2), positions 16 (i % 2)
+            union Frag4 {
+                s16x4 q[2];
+                i32x4 v;
+            } vf[kAhead];
+            auto read = [&](int i, int e) {
+                return __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                    (lds_s16x4*)(V + (own ^ 64 * (i / 2)) + (16 * (i % 2) + 8 * e) * U * 16));
+            };
 #pragma unroll
-            for (int dt = 0; dt < HD / 32; ++dt)
+            for (int i = 0; i < kAhead; ++i)
 #pragma unroll
-                for (int ks = 0; ks < 2; ++ks) {
-                    union {
-                        s16x4 q[2];
-                        i32x4 v;
-                    } vf;
+                for (int e = 0; e < 2; ++e) vf[i].q[e] = read(i, e);
 #pragma unroll
-                    for (int e = 0; e < 2; ++e)
-                        vf.q[e] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                            (lds_s16x4*)(V + (own ^ 64 * dt) + (16 * ks + 8 * e) * U * 16));
-                    if constexpr (edge) {
+            for (int i = 0; i < N; ++i) {
+                i32x4 v = vf[i % kAhead].v;
+                if constexpr (edge) {
 #pragma unroll
-                        for (int k = 0; k < 4; ++k) {
-                            const uint32_t z = vf.v[k];
-                            const bool lo_bad = (z & F::kInf) == F::kInf, hi_bad = (z >> 16 & F::kInf) == F::kInf;
-                            bad |= lo_bad || hi_bad;
-                            vf.v[k] = z & (lo_bad ? 0xffff0000u : ~0u) & (hi_bad ? 0xffffu : ~0u);
-                        }
+                    for (int k = 0; k < 4; ++k) {
+                        const uint32_t z = v[k];
+                        const bool lo_bad = (z & F::kInf) == F::kInf, hi_bad = (z >> 16 & F::kInf) == F::kInf;
+                        bad |= lo_bad || hi_bad;
+                        v[k] = z & (lo_bad ? 0xffff0000u : ~0u) & (hi_bad ? 0xffffu : ~0u);
                     }
-                    o[dt] = F::mfma(vf.v, w.hi[ks], o[dt]);
-                    if constexpr (kTwo) o[dt] = F::mfma(vf.v, w.lo[ks], o[dt]);
                 }
+                o[i / 2] = F::mfma(v, __builtin_bit_cast(i32x4, w.hi[i % 2]), o[i / 2]);
+                if constexpr (kTwo) o[i / 2] = F::mfma(v, __builtin_bit_cast(i32x4, w.lo[i % 2]), o[i / 2]);
+                pin(o[i / 2]);
+                if (i + kAhead < N)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) vf[i % kAhead].q[e] = read(i + kAhead, e);
+                side(i);
+                __builtin_amdgcn_sched_barrier(0);
+            }
             if (edge && __any(bad)) {
                 const C* Ve = reinterpret_cast<const C*>(Vt);
 #pragma unroll 1
@@ -386,76 +434,84 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void tree_attn_kernel(TreeA
         if constexpr (WP == 1) {
             // every wave by itself: K of its next tile comes while this one's V is used, and the other way round
             i32x4 *K = K_s + wave * kTile, *V = V_s + wave * kTile;
-            uint32_t next = 0;
+            int next = 0;
             if (ua < ub) {
-                const uint32_t rows = entry(ua, wave);
-                next = entry(min(ua + 1, ub - 1), wave);
-                load(p.k, K, rows, false);
+                const uint32_t rows = row_of(page_of(ua, wave), ua, wave);
+                next = page_of(min(ua + 1, ub - 1), wave);
+                load(p.k, K, rows, false, page_runs && ua < u_edge);
                 load_q();
                 asm volatile("" ::: "memory");
-                load(p.v, V, rows, true);
+                load(p.v, V, rows, true, page_runs && ua < u_edge);
             }
             auto rounds = [&]<bool edge>(std::bool_constant<edge> e, int from, int to) {
                 for (int u = from; u < to; ++u) {
-                    const bool more = u + 1 < ub;
+                    const bool more = u + 1 < ub, runs = page_runs && u + 1 < u_edge;
                     f32x16 sn[1];
                     uint32_t vis = ~0u;
                     Weights w;
                     // all but the last kLoads loads, V's
                     asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kLoads) : "memory");
-                    const uint32_t rows = next;
-                    next = entry(min(u + 2, ub - 1), wave);
+                    const uint32_t rows = row_of(next, min(u + 1, ub - 1), wave);
+                    next = page_of(min(u + 2, ub - 1), wave);
                     asm volatile("" ::: "memory");
-                    scores(K, sn[0]);
+                    scores(K, sn);
                     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-                    if (more) load(p.k, K, rows, false);
+                    if (more) load(p.k, K, rows, false, runs);
                     if constexpr (edge) hide(sn[0], vis = seen32(p, s, j, u * kUnit + 32 * wave));
                     raise(sn);
-                    weights(sn[0], w);
+                    weights(sn[0], w, level());
                     // all but the next K's
                     if (more)
                         asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kLoads) : "memory");
                     else
                         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-                    output(e, V, w, vis);
+                    output(e, V, w, vis, [](int) {});
                     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-                    if (more) load(p.v, V, rows, true);
+                    if (more) load(p.v, V, rows, true, runs);
                 }
             };
             rounds(std::false_type(), ua, u_edge);
             rounds(std::true_type(), u_edge, ub);
         } else {
             // wave w brings tile w % 2 of K (w < 2) or V: the next round's while this one is computed
-            const void* pool = wave < 2 ? p.k : p.v;
-            i32x4* mem = (wave < 2 ? K_s : V_s) + (wave & 1) * kTile;
-            uint32_t next = 0;
+            const bool is_v = wave >= 2;
+            const void* pool = is_v ? p.v : p.k;
+            i32x4* mem = (is_v ? V_s : K_s) + (wave & 1) * kTile;
+            int next = 0;
             if (ua < ub) {
-                load(pool, mem + (ua & 1) * 2 * kTile, entry(ua, wave & 1), wave >= 2);
-                next = entry(min(ua + 1, ub - 1), wave & 1);
+                load(pool, mem + (ua & 1) * 2 * kTile, row_of(page_of(ua, wave & 1), ua, wave & 1), is_v, page_runs && ua < u_edge);
+                next = page_of(min(ua + 1, ub - 1), wave & 1);
             }
             load_q();
             auto rounds = [&]<bool edge>(std::bool_constant<edge> e, int from, int to) {
                 for (int u = from; u < to; ++u) {
                     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-                    if (u + 1 < ub) {
-                        load(pool, mem + ((u + 1) & 1) * 2 * kTile, next, wave >= 2);
-                        next = entry(min(u + 2, ub - 1), wave & 1);
-                    }
+                    const uint32_t rows = row_of(next, min(u + 1, ub - 1), wave & 1);
+                    next = page_of(min(u + 2, ub - 1), wave & 1);
+                    if (u + 1 < ub) load(pool, mem + ((u + 1) & 1) * 2 * kTile, rows, is_v, page_runs && u + 1 < u_edge);
                     const i32x4 *K = K_s + ((u & 1) * 2 + ws * NT) * kTile, *V = V_s + ((u & 1) * 2 + ws * NT) * kTile;
                     f32x16 sn[NT];
                     uint32_t vis[NT];
                     Weights w[NT];
+                    scores(K, sn);
 #pragma unroll
                     for (int a = 0; a < NT; ++a) {
-                        scores(K + a * kTile, sn[a]);
                         vis[a] = ~0u;
                         if constexpr (edge) hide(sn[a], vis[a] = seen32(p, s, j, u * kUnit + 32 * (ws * NT + a)));
                     }
                     raise(sn);
+                    const float sub = level();
+                    weights(sn[0], w[0], sub);
+                    if constexpr (NT == 2) {
+                        // the second tile's weights under the first one's products
+                        output(e, V, w[0], vis[0], [&](int i) {
 #pragma unroll
-                    for (int a = 0; a < NT; ++a) weights(sn[a], w[a]);
-#pragma unroll
-                    for (int a = 0; a < NT; ++a) output(e, V + a * kTile, w[a], vis[a]);
+                            for (int k = 8 * i / (HD / 16); k < 8 * (i + 1) / (HD / 16); ++k) weights2(sn[1], w[1], sub, k);
+                        });
+                        output(e, V + kTile, w[1], vis[1], [](int) {});
+                    } else {
+                        output(e, V, w[0], vis[0], [](int) {});
+                    }
                 }
             };
             rounds(std::false_type(), ua, u_edge);
