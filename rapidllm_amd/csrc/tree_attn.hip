@@ -102,8 +102,7 @@ __device__ inline Lanes lanes_at(const TreeArgs& p, int b0, int before) {
     }
     f.units = f.s.n ? (f.s.ctx + f.s.n + p.unit - 1) / p.unit : 0;
     f.end = f.units * p.nkv;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
+    for (int o = 1; o < 64 && o < p.n_seq; o <<= 1) {  // lanes past the last sequence: any value
         const int x = __shfl_up(f.end, o, 64);
         if ((threadIdx.x & 63) >= o) f.end += x;
     }
@@ -114,8 +113,8 @@ __device__ inline int lane_value(int v, int lane) { return __builtin_amdgcn_read
 // Units of a workgroup: workgroup c has units c * per up to (c + 1) * per of the first 64 sequences' f and
 // the rest.
 __device__ inline int total_units(const TreeArgs& p, const Lanes& f) {
-    int total = lane_value(f.end, 63);
-    for (int b0 = 64; b0 < p.n_seq; b0 += 64) total = lane_value(lanes_at(p, b0, total).end, 63);
+    int total = lane_value(f.end, min(p.n_seq, 64) - 1);
+    for (int b0 = 64; b0 < p.n_seq; b0 += 64) total = lane_value(lanes_at(p, b0, total).end, min(p.n_seq - b0, 64) - 1);
     return total;
 }
 
@@ -266,21 +265,24 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void tree_attn_kernel(TreeA
         };
         const bool page_runs = p.page >= kPerLoad;
 
-        // q: this lane's column of the operand, dims 16 st + 8 h ..
+        // q: this lane's column of the operand, dims 16 st + 8 h ..  Asked for before everything else, split
+        // while K and V come.
+        typename Vec4<T>::type qr[HD / 8];
         i32x4 qh[HD / 16], ql[kTwo ? HD / 16 : 1];
-        auto load_q = [&] {
+        {
             const T* src = static_cast<const T*>(p.q) + row * p.q_row + head * p.q_head + 8 * h;
+#pragma unroll
+            for (int i = 0; i < HD / 8; ++i) qr[i] = *reinterpret_cast<const typename Vec4<T>::type*>(src + 16 * (i / 2) + 4 * (i % 2));
+        }
+        auto split_q = [&] {
 #pragma unroll
             for (int st = 0; st < HD / 16; ++st) {
                 typename F::type hi, lo;
 #pragma unroll
-                for (int e = 0; e < 8; e += 4) {
-                    const f32x4 v = load4(src + 16 * st + e);
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        hi[e + k] = static_cast<C>(v[k]);
-                        if constexpr (kTwo) lo[e + k] = static_cast<C>(v[k] - static_cast<float>(hi[e + k]));
-                    }
+                for (int e = 0; e < 8; ++e) {
+                    const float v = static_cast<float>(qr[2 * st + e / 4][e % 4]);
+                    hi[e] = static_cast<C>(v);
+                    if constexpr (kTwo) lo[e] = static_cast<C>(v - static_cast<float>(hi[e]));
                 }
                 qh[st] = __builtin_bit_cast(i32x4, hi);
                 if constexpr (kTwo) ql[st] = __builtin_bit_cast(i32x4, lo);
@@ -439,10 +441,10 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void tree_attn_kernel(TreeA
                 const uint32_t rows = row_of(page_of(ua, wave), ua, wave);
                 next = page_of(min(ua + 1, ub - 1), wave);
                 load(p.k, K, rows, false, page_runs && ua < u_edge);
-                load_q();
                 asm volatile("" ::: "memory");
                 load(p.v, V, rows, true, page_runs && ua < u_edge);
             }
+            split_q();
             auto rounds = [&]<bool edge>(std::bool_constant<edge> e, int from, int to) {
                 for (int u = from; u < to; ++u) {
                     const bool more = u + 1 < ub, runs = page_runs && u + 1 < u_edge;
@@ -482,7 +484,7 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void tree_attn_kernel(TreeA
                 load(pool, mem + (ua & 1) * 2 * kTile, row_of(page_of(ua, wave & 1), ua, wave & 1), is_v, page_runs && ua < u_edge);
                 next = page_of(min(ua + 1, ub - 1), wave & 1);
             }
-            load_q();
+            split_q();
             auto rounds = [&]<bool edge>(std::bool_constant<edge> e, int from, int to) {
                 for (int u = from; u < to; ++u) {
                     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
@@ -524,6 +526,7 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void tree_attn_kernel(TreeA
         char* O_s = reinterpret_cast<char*>((wave < 2 ? K_s : V_s) + (wave & 1) * (2 * kTile));
         const int oaddr = opaque((col * (HD / 4) + (h ^ (col & 15))) * 16);
         if (h == 0) ml_s[wave][col] = make_float2(m, l);
+        if (pair0 + 32 * wp + col < pairs)
 #pragma unroll
         for (int dt = 0; dt < HD / 32; ++dt)
 #pragma unroll
@@ -558,7 +561,7 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void tree_attn_kernel(TreeA
                 if (od == 0) p.part_ml[part * (32 * WP) + q] = make_float2(M, L2);
             }
         }
-        __syncthreads();
+        if (t < t1) __syncthreads();
     }
 }
 
@@ -604,12 +607,22 @@ __global__ __launch_bounds__(256) void tree_attn_join_kernel(TreeArgs p, int til
             L = L * old + wave_sum(lw);
             acc = acc * old;
             const int n = min(64, wz - w0 + 1);
-#pragma unroll 4
-            for (int i = grp; i < n; i += kGroups) {
-                const float fw = __shfl(wt, i, 64);
-                const size_t at = ((static_cast<size_t>(w0 + i) * p.q_tiles + qt) * 2 + ((w0 + i) * per < t0)) * tile + q;
-                const f32x4 o = *reinterpret_cast<const f32x4*>(p.part_o + at * HD + 4 * od);
-                if (fw != 0.f) acc += o * fw;
+            for (int i0 = grp; i0 < n; i0 += 8 * kGroups) {
+                f32x4 o[8];
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    const int w = w0 + min(i0 + k * kGroups, n - 1);
+                    const size_t at = ((static_cast<size_t>(w) * p.q_tiles + qt) * 2 + (w * per < t0)) * tile + q;
+                    o[k] = *reinterpret_cast<const f32x4*>(p.part_o + at * HD + 4 * od);
+                }
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    // a part without weight may hold anything
+                    const float fw = __shfl(wt, min(i0 + k * kGroups, n - 1), 64);
+                    const bool on = i0 + k * kGroups < n && fw != 0.f;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) acc[e] = on ? fmaf(o[k][e], fw, acc[e]) : acc[e];
+                }
             }
         }
     }
