@@ -415,7 +415,7 @@ int rl_hip_tree_accept(const RlPagedCache* cache, const int* table, int table_wi
  * probability 0; among logits of +infinity the weights are 1 and all others 0.
  * Weights are sums of integers, in units of at most 2^-44 of the largest up to a vocab of
  * 2^18 (above, vocab * 2^-62), so the result does not depend on the order of the work;
- * tokens below half a unit are never picked.  vocab <= 2^24.  workspace:
+ * tokens below half a unit are never picked.  vocab <= 2^24, rows <= 2^20.  workspace:
  * rl_hip_sample_workspace_bytes; calls that overlap in time need one each. */
 size_t rl_hip_sample_workspace_bytes(int rows, int vocab);
 int rl_hip_sample_rows(int dtype, const void* logits, int64_t ld, int rows, int vocab, const float* temperature,

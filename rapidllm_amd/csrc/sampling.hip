@@ -1,13 +1,19 @@
 // sampling.hip -- one token per row of logits: temperature, top-k, top-p, min-p, from given random
 // numbers.
 //
-// With M the row's maximum and w = exp((z - M) / T), what top-k and top-p keep is a prefix of the
-// order (larger z first, equal z by lower index), so it is told by one element, the last kept.
-// That element is found without sorting: a histogram of (M - z) / T gives the bin it is in and
-// the count and mass before the bin, and only the bin's own elements are put in order.
-// Masses are integers (w in units of 2^-44 of the largest), so that sums are exact in any order
-// and every kernel sees the same element the same way.
+// With M the row's maximum and w = exp((z - M) / T) = 2^-depth, what top-k and top-p keep is a prefix
+// of the order (larger z first, equal z by lower index), so it is told by one element, the last kept.
+// That element is found without sorting: a histogram over the depth gives the bin it is in and the
+// count and mass before the bin, and only that bin's own elements are put in order.  The token
+// follows from the masses of tiles of 512 logits, then from one tile's logits.
+// Masses are integers (w in units of 2^-44 of the largest), so that sums are exact in any order and
+// every kernel sees the same element the same way.
+// Four launches, the first three with many workgroups per row: maximum; histogram (rows without
+// top-k and top-p: the tiles' masses already); the tiles' surely kept masses and a list of the
+// border bins' elements (such rows skip it); the choice.  One workgroup per row doing all of it took
+// 344 us for one row of 248320 logits, 633 us for 128.
 #include <algorithm>
+#include <cmath>
 
 #include "paged.h"
 
@@ -15,328 +21,584 @@ using namespace rl;
 
 namespace {
 
+typedef unsigned long long u64;
+
+constexpr int kTile = 512;             // logits of a wave at a time, 8 per lane
 constexpr int kBins = 2048;
-constexpr double kBinsPerUnit = 64.0;  // bins cover weights down to exp(-32) < 2^-45
-constexpr int kList = 2048;            // elements of one bin put in order in shared memory
-constexpr int kThreads = 1024;
+constexpr double kBinsPerUnit = 44.0;  // bins of depth
+constexpr double kDepth = 45.0;        // weights from 2^-45 down are no unit
+constexpr int kList = 4096;            // elements of the border bins that are listed
+constexpr int kPick = 1024;            // threads of the last launch
 
 struct SampleArgs {
     const void* logits;
     int64_t ld;
     int V, shift;  // masses in units of 2^-shift
+    int chunk, chunks, tiles;  // logits of a workgroup, workgroups and tiles of a row
     const float *temperature, *top_p, *min_p, *u;
     const int* top_k;
     int* idx;
     float* prob;
+    // workspace, per row
+    float* cmax;   // [chunks]
+    unsigned* cnt; // [kBins] + the list's length
+    u64* mass;     // [kBins]
+    u64* tmass;    // [tiles]
+    u64* list;     // [kList] keys
+    bool wide;     // rows start at 16 bytes
 };
 
 // Larger first, equal ones by index.
-__device__ inline uint64_t order_key(float z, int i) {
+__device__ inline u64 order_key(float z, int i) {
     const uint32_t b = __float_as_uint(z);
     const uint32_t up = b >> 31 ? ~b : b | 0x80000000u;
-    return static_cast<uint64_t>(~up) << 32 | static_cast<uint32_t>(i);
+    return static_cast<u64>(~up) << 32 | static_cast<uint32_t>(i);
 }
-__device__ inline float key_value(uint64_t key) {
+__device__ inline float key_value(u64 key) {
     const uint32_t up = ~static_cast<uint32_t>(key >> 32);
     return __uint_as_float(up >> 31 ? up & 0x7fffffffu : ~up);
 }
 
-template <class T>
-__device__ inline float logit(const T* row, int i) {
-    const float z = static_cast<float>(row[i]) + 0.f;  // -0 becomes +0: they are equal
+// -0 becomes +0 (they are equal), NaN -infinity
+__device__ inline float clean(float z) {
+    z += 0.f;
     return z != z ? -INFINITY : z;
 }
+// logits i .. i + 7, -infinity past the row
+template <class T>
+__device__ inline void load8(const T* row, int i, int end, bool wide, float (&z)[8]) {
+    if (wide && i + 8 <= end) {
+        typedef T T8 __attribute__((ext_vector_type(16 / sizeof(T))));
+#pragma unroll
+        for (int k = 0; k < 8; k += 16 / sizeof(T)) {
+            const T8 v = *reinterpret_cast<const T8*>(row + i + k);
+#pragma unroll
+            for (unsigned e = 0; e < 16 / sizeof(T); ++e) z[k + e] = clean(static_cast<float>(v[e]));
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) z[k] = i + k < end ? clean(static_cast<float>(row[i + k])) : -INFINITY;
+    }
+}
 
+// 2^r for |r| <= 1/2, to 2^-50: the exponential's series to the 12th power
+__device__ inline double exp2_small(double r) {
+    const double x = r * 0.693147180559945309417;
+    double y = 1.0 / 479001600.0;
+    y = fma(y, x, 1.0 / 39916800.0);
+    y = fma(y, x, 1.0 / 3628800.0);
+    y = fma(y, x, 1.0 / 362880.0);
+    y = fma(y, x, 1.0 / 40320.0);
+    y = fma(y, x, 1.0 / 5040.0);
+    y = fma(y, x, 1.0 / 720.0);
+    y = fma(y, x, 1.0 / 120.0);
+    y = fma(y, x, 1.0 / 24.0);
+    y = fma(y, x, 1.0 / 6.0);
+    y = fma(y, x, 0.5);
+    y = fma(y, x, 1.0);
+    return fma(y, x, 1.0);
+}
+
+// A row's settings, and what its logits weigh.
 struct Row {
     float M;
-    double inv_t, unit, min_p;
-    // depth (M - z) / T, >= 0; 1e9 for what has no weight at all
+    double scale, min_p, top_p;
+    int shift, top_k;  // 0: off
+    bool greedy, use_p;
+    __device__ bool filters() const { return top_k || use_p; }
+    // (M - z) / (T ln 2), >= 0; past kDepth for what has no weight at all
     __device__ double depth(float z) const {
         if (z == M) return 0.0;
         if (z == -INFINITY || M == INFINITY) return 1e9;
-        return (static_cast<double>(M) - static_cast<double>(z)) * inv_t;
+        return (static_cast<double>(M) - static_cast<double>(z)) * scale;
     }
-    __device__ double weight(double depth) const { return depth < 32.0 ? exp(-depth) : 0.0; }
-    __device__ unsigned long long mass(double w) const { return static_cast<unsigned long long>(rint(w * unit)); }
-    __device__ int bin(double depth) const { return static_cast<int>(depth * kBinsPerUnit); }
+    // everything below has a depth past kDepth, or past the bin's end (one step of z below, for the rounding)
+    __device__ float below(double depth) const {
+        if (M == INFINITY) return M;
+        const double z = static_cast<double>(M) - depth / scale;
+        return scale > 0.0 && z > -3e38 ? nextafterf(nextafterf(static_cast<float>(z), -INFINITY), -INFINITY) : -INFINITY;
+    }
+    __device__ double weight(double depth) const {
+        const double n = rint(depth);
+        return ldexp(exp2_small(n - depth), -static_cast<int>(n));
+    }
+    // 2^52 + w 2^shift holds the rounded number in its low bits
+    __device__ u64 mass_of(double w) const {
+        const double x = ldexp(w, shift) + 4503599627370496.0;
+        return static_cast<u64>(__double_as_longlong(x)) & 0xfffffffffffffull;
+    }
+    __device__ u64 mass(double depth) const { return depth < kDepth ? mass_of(weight(depth)) : 0; }
+    // with min_p: nothing of what falls under it
+    __device__ u64 kept(double depth) const {
+        if (depth >= kDepth) return 0;
+        const double w = weight(depth);
+        return w >= min_p ? mass_of(w) : 0;
+    }
+    __device__ static int bin(double depth) { return static_cast<int>(depth * kBinsPerUnit); }
 };
 
+__device__ inline Row settings(const SampleArgs& p, int row, float M) {
+    Row r;
+    r.M = M;
+    const float t = p.temperature ? p.temperature[row] : 1.f;
+    r.greedy = !(t > 0.f) || M == -INFINITY;
+    r.scale = 1.0 / static_cast<double>(t) * 1.44269504088896340736;
+    const float mp = p.min_p ? p.min_p[row] : 0.f;
+    r.min_p = mp > 0.f ? fminf(mp, 1.f) : 0.0;
+    const int k = p.top_k ? p.top_k[row] : 0;
+    r.top_k = k > 0 && k < p.V ? k : 0;
+    const float tp = p.top_p ? p.top_p[row] : 1.f;
+    r.use_p = tp < 1.f;
+    r.top_p = tp;
+    r.shift = p.shift;
+    return r;
+}
+
+// Sum over the waves before, and of all; every thread calls it.  part: one per wave.
 template <class T>
-__device__ inline T wave_scan(T v) {
-    const int lane = threadIdx.x & 63;
+__device__ inline T block_scan(T v, T* part, T* total = nullptr) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
         const T x = __shfl_up(v, o, 64);
         if (lane >= o) v += x;
     }
-    return v;
-}
-// inclusive sum over the workgroup; all threads call it
-template <class T>
-__device__ inline T block_scan(T v, T* part) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    v = wave_scan(v);
     __syncthreads();
     if (lane == 63) part[wave] = v;
     __syncthreads();
-    T before = 0;
-    for (int w = 0; w < wave; ++w) before += part[w];
+    T before = 0, all = 0;
+    for (int w = 0; w < waves; ++w) {
+        if (w < wave) before += part[w];
+        all += part[w];
+    }
+    if (total) *total = all;
     return v + before;
 }
+__device__ inline float block_max(float v, float* part) {
+    v = wave_max(v);
+    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = part[0];
+    for (unsigned w = 1; w < blockDim.x >> 6; ++w) v = fmaxf(v, part[w]);
+    return v;
+}
+__device__ inline float row_max(const SampleArgs& p, int row, float* part) {
+    float m = -INFINITY;
+    for (int i = threadIdx.x; i < p.chunks; i += blockDim.x) m = fmaxf(m, p.cmax[static_cast<size_t>(row) * p.chunks + i]);
+    return block_max(m, part);
+}
 
-typedef unsigned long long u64;
+template <class T>
+struct Part {  // a workgroup's part of a row
+    int row, chunk, begin, end;
+    const T* z;
+};
+template <class T>
+__device__ inline Part<T> part_of(const SampleArgs& p) {
+    Part<T> a;
+    a.row = blockIdx.x / p.chunks, a.chunk = blockIdx.x % p.chunks;
+    a.begin = a.chunk * p.chunk, a.end = min(p.V, a.begin + p.chunk);
+    a.z = static_cast<const T*>(p.logits) + a.row * p.ld;
+    return a;
+}
 
-struct Shared {
-    unsigned cnt[kBins];
-    u64 mass[kBins];
-    u64 key[kList];
-    u64 w[kList];
-    u64 part[kThreads / 64];
-    unsigned cpart[kThreads / 64];
-    uint64_t best[kThreads / 64];
-    int n;
-    // what a search found
-    int bin;
+template <class T>
+__global__ __launch_bounds__(256) void sample_max_kernel(SampleArgs p) {
+    __shared__ float part_s[4];
+    const Part<T> a = part_of<T>(p);
+    float m = -INFINITY;
+    for (int i = a.begin + 8 * threadIdx.x; i < a.end; i += 8 * 256) {
+        float z[8];
+        load8(a.z, i, a.end, p.wide, z);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) m = fmaxf(m, z[e]);
+    }
+    m = block_max(m, part_s);
+    if (threadIdx.x == 0) p.cmax[static_cast<size_t>(a.row) * p.chunks + a.chunk] = m;
+    // the next launches' histogram and list start empty
+    const size_t row = a.row;
+    for (int i = a.chunk * 256 + threadIdx.x; i <= kBins; i += 256 * p.chunks) {
+        p.cnt[row * (kBins + 1) + i] = 0;
+        if (i < kBins) p.mass[row * kBins + i] = 0;
+    }
+}
+
+__device__ inline u64 wave_sum64(u64 v) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+    return v;
+}
+
+template <class T>
+__global__ __launch_bounds__(256) void sample_hist_kernel(SampleArgs p) {
+    __shared__ float part_s[4];
+    __shared__ unsigned cnt_s[kBins];
+    __shared__ u64 mass_s[kBins];
+    const Part<T> a = part_of<T>(p);
+    const Row r = settings(p, a.row, row_max(p, a.row, part_s));
+    if (r.greedy) return;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const float low = r.below(kDepth);
+    if (!r.filters()) {
+        for (int t = a.begin / kTile + wave; t * kTile < a.end; t += 4) {
+            float z[8];
+            load8(a.z, t * kTile + 8 * lane, a.end, p.wide, z);
+            u64 m = 0;
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (z[e] >= low) m += r.kept(r.depth(z[e]));
+            m = wave_sum64(m);
+            if (lane == 0) p.tmass[static_cast<size_t>(a.row) * p.tiles + t] = m;
+        }
+        return;
+    }
+    for (int i = threadIdx.x; i < kBins; i += 256) {
+        cnt_s[i] = 0;
+        mass_s[i] = 0;
+    }
+    __syncthreads();
+    for (int i = a.begin + 8 * threadIdx.x; i < a.end; i += 8 * 256) {
+        float z[8];
+        load8(a.z, i, a.end, p.wide, z);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            if (!(z[e] >= low)) continue;
+            const double d = r.depth(z[e]);
+            if (d >= kDepth) continue;
+            if (r.top_k) atomicAdd(&cnt_s[r.bin(d)], 1u);
+            if (r.use_p) atomicAdd(&mass_s[r.bin(d)], r.mass(d));
+        }
+    }
+    __syncthreads();
+    const size_t row = a.row;
+    for (int i = threadIdx.x; i < kBins; i += 256) {
+        if (r.top_k && cnt_s[i]) atomicAdd(&p.cnt[row * (kBins + 1) + i], cnt_s[i]);
+        if (r.use_p && mass_s[i]) atomicAdd(&p.mass[row * kBins + i], mass_s[i]);
+    }
+}
+
+// The bins in which top-k and top-p end: everything before `sure` is kept, nothing past `top`, and top-k
+// itself ends in k_bin (kBins: it cuts nothing off).
+struct Borders {
+    int sure, top, k_bin;
+    unsigned k_before;  // elements before k_bin
+    u64 k_mass, all;    // mass before k_bin (with top-p), of all bins
+};
+struct BorderShared {
+    unsigned cpart[16];
+    u64 part[16];
+    int k_bin, lo, hi;
+    unsigned k_before;
+    u64 k_mass, k_own;
+};
+template <int kThreads>
+__device__ Borders borders(const SampleArgs& p, int row_, const Row& r, BorderShared& sh) {
+    constexpr int E = kBins / kThreads;
+    const int tid = threadIdx.x;
+    const size_t row = row_;
+    unsigned c[E], cs = 0, ct = 0;
+    u64 m[E], ms = 0, mt = 0;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        c[e] = r.top_k ? p.cnt[row * (kBins + 1) + tid * E + e] : 0;
+        m[e] = r.use_p ? p.mass[row * kBins + tid * E + e] : 0;
+        cs += c[e];
+        ms += m[e];
+    }
+    if (tid == 0) sh.k_bin = kBins, sh.lo = sh.hi = kBins;
+    const unsigned c0 = block_scan(cs, sh.cpart, &ct) - cs;
+    const u64 m0 = block_scan(ms, sh.part, &mt) - ms;
+    if (r.top_k && static_cast<unsigned>(r.top_k) < ct) {
+        unsigned cb = c0;
+        u64 mb = m0;
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            if (cb < static_cast<unsigned>(r.top_k) && static_cast<unsigned>(r.top_k) <= cb + c[e]) {
+                sh.k_bin = tid * E + e;
+                sh.k_before = cb;
+                sh.k_mass = mb;
+                sh.k_own = m[e];
+            }
+            cb += c[e];
+            mb += m[e];
+        }
+    }
+    __syncthreads();
+    Borders b;
+    b.k_bin = sh.k_bin;
+    b.k_before = sh.k_before;
+    b.k_mass = sh.k_mass;
+    b.all = mt;
+    b.sure = b.top = b.k_bin;
+    if (r.use_p) {
+        // top-k leaves between k_mass and that with all of its last bin
+        const u64 least = b.k_bin < kBins ? b.k_mass : mt, most = b.k_bin < kBins ? b.k_mass + sh.k_own : mt;
+        const double lo = fmax(r.top_p * static_cast<double>(least), 0.5), hi = fmax(r.top_p * static_cast<double>(most), 0.5);
+        u64 mb = m0;
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            const double x = static_cast<double>(mb), y = static_cast<double>(mb + m[e]);
+            if (x < lo && y >= lo) sh.lo = tid * E + e;
+            if (x < hi && y >= hi) sh.hi = tid * E + e;
+            mb += m[e];
+        }
+        __syncthreads();
+        b.sure = min(sh.lo, b.k_bin);
+        b.top = min(sh.hi, b.k_bin);
+    }
+    return b;
+}
+
+template <class T>
+__global__ __launch_bounds__(256) void sample_list_kernel(SampleArgs p) {
+    __shared__ float part_s[4];
+    __shared__ BorderShared sh;
+    const Part<T> a = part_of<T>(p);
+    const Row r = settings(p, a.row, row_max(p, a.row, part_s));
+    if (r.greedy || !r.filters()) return;
+    const Borders b = borders<256>(p, a.row, r, sh);
+    const int last = b.k_bin < kBins ? b.k_bin : b.top;  // the last bin looked at
+    const float low = r.below(fmin((last + 1) / kBinsPerUnit, kDepth));
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const size_t row = a.row;
+    for (int t = a.begin / kTile + wave; t * kTile < a.end; t += 4) {
+        float z[8];
+        const int i = t * kTile + 8 * lane;
+        load8(a.z, i, a.end, p.wide, z);
+        u64 m = 0;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            if (!(z[e] >= low)) continue;
+            const double d = r.depth(z[e]);
+            if (d >= kDepth) continue;
+            const int bin = r.bin(d);
+            if (bin < b.sure) {
+                m += r.kept(d);
+            } else if (bin <= b.top || bin == b.k_bin) {
+                const unsigned at = atomicAdd(&p.cnt[row * (kBins + 1) + kBins], 1u);
+                if (at < kList) p.list[row * kList + at] = order_key(z[e], i + e);
+            }
+        }
+        m = wave_sum64(m);
+        if (lane == 0) p.tmass[row * p.tiles + t] = m;
+    }
+}
+
+struct PickShared {
+    BorderShared b;
+    float fpart[kPick / 64];
+    u64 part[kPick / 64];
+    u64 key[kList];   // the list; where it does not hold the border bins, the radix search's counts
+    u64 range[kPick]; // masses of equal shares of the row
+    u64 dig_n[256], dig_m[256];
+    u64 found_key, found_upto, before_m;
     unsigned before_n;
-    u64 before_m, found_key, found_m;
+    int digit, n, at;
 };
 
-// Which element of the row ends the prefix: the `want_n`th of the order, or the first up to which
-// want_m of mass stands; elements past `last` do not count.  Histograms in sh; before the call the
-// bin, before_n and before_m are known.  Returns the element's key, its mass included in *upto.
-template <class T>
-__device__ uint64_t find_in_bin(const SampleArgs& p, const T* row, const Row& r, Shared& sh, uint64_t last, unsigned want_n,
-                                double want_m, u64* upto) {
-    const int tid = threadIdx.x;
-    const int bin = sh.bin;
-    const unsigned before_n = sh.before_n;
-    const u64 before_m = sh.before_m;
-    const unsigned n_bin = sh.cnt[bin];
-    if (n_bin <= kList) {
-        __syncthreads();
-        if (tid == 0) sh.n = 0;
-        __syncthreads();
-        for (int i = tid; i < p.V; i += kThreads) {
-            const float z = logit(row, i);
-            const double d = r.depth(z);
-            if (d >= 32.0 || r.bin(d) != bin) continue;
-            const uint64_t key = order_key(z, i);
-            const u64 m = r.mass(r.weight(d));
-            if (m == 0 || key > last) continue;
-            const int at = atomicAdd(&sh.n, 1);
-            sh.key[at] = key;
-            sh.w[at] = m;
-        }
-        __syncthreads();
-        const int n = sh.n;
-        for (int e = tid; e < n; e += kThreads) {
-            const uint64_t key = sh.key[e];
-            unsigned rank = before_n;
-            u64 m = before_m;
-            for (int j = 0; j < n; ++j)
-                if (sh.key[j] < key) {
-                    ++rank;
-                    m += sh.w[j];
-                }
-            const bool hit = want_n ? rank + 1 == want_n
-                                    : static_cast<double>(m) < want_m && static_cast<double>(m + sh.w[e]) >= want_m;
-            if (hit) {
-                sh.found_key = key;
-                sh.found_m = m + sh.w[e];
-            }
-        }
-        __syncthreads();
-        *upto = sh.found_m;
-        return sh.found_key;
-    }
-    // many elements in one bin (flat or repeated logits): eight bits of the key at a time
-    uint64_t prefix = 0;
-    unsigned base_n = before_n;
-    u64 base_m = before_m;
+// Which of the elements that `each` hands out ends the prefix: the one with `want_n` up to it (before_n stand
+// before all of them), or else the first up to which want_m of mass stands.  The key of it, *upto the mass up to it.
+template <class Each>
+__device__ u64 find_last(PickShared& sh, Each each, unsigned before_n, u64 before_m, unsigned want_n, double want_m, u64* upto) {
+    // eight bits of the key at a time
+    u64 prefix = 0;
     for (int shift = 56; shift >= 0; shift -= 8) {
         __syncthreads();
-        for (int i = tid; i < 256; i += kThreads) {
-            sh.key[i] = 0;
-            sh.w[i] = 0;
+        if (threadIdx.x < 256) sh.dig_n[threadIdx.x] = sh.dig_m[threadIdx.x] = 0;
+        __syncthreads();
+        each([&](u64 key, u64 m) {
+            if (shift < 56 && (key ^ prefix) >> (shift + 8)) return;
+            atomicAdd(&sh.dig_n[key >> shift & 255], 1ull);
+            atomicAdd(&sh.dig_m[key >> shift & 255], m);
+        });
+        __syncthreads();
+        u64 n = 0, m = 0;
+        if (threadIdx.x < 256) n = sh.dig_n[threadIdx.x], m = sh.dig_m[threadIdx.x];
+        const u64 ni = block_scan(n, sh.part) + before_n, mi = block_scan(m, sh.part) + before_m;
+        const bool hit = want_n ? ni - n < want_n && want_n <= ni
+                                : static_cast<double>(mi - m) < want_m && static_cast<double>(mi) >= want_m;
+        if (n && hit) {
+            sh.digit = threadIdx.x;
+            sh.before_n = static_cast<unsigned>(ni - n);
+            sh.before_m = mi - m;
+            sh.found_upto = mi;
         }
         __syncthreads();
-        for (int i = tid; i < p.V; i += kThreads) {
-            const float z = logit(row, i);
-            const double d = r.depth(z);
-            if (d >= 32.0 || r.bin(d) != bin) continue;
-            const uint64_t key = order_key(z, i);
-            const u64 m = r.mass(r.weight(d));
-            if (m == 0 || key > last || (shift < 56 && (key ^ prefix) >> (shift + 8))) continue;
-            atomicAdd(reinterpret_cast<u64*>(&sh.key[key >> shift & 255]), 1ull);
-            atomicAdd(&sh.w[key >> shift & 255], m);
-        }
-        __syncthreads();
-        if (tid == 0) {
-            u64 c = base_n, m = base_m;
-            int digit = 0;
-            for (; digit < 256; ++digit) {
-                const bool hit = want_n ? c + sh.key[digit] >= want_n : static_cast<double>(m + sh.w[digit]) >= want_m;
-                if (sh.key[digit] && hit) break;
-                c += sh.key[digit];
-                m += sh.w[digit];
-            }
-            sh.before_n = static_cast<unsigned>(c);
-            sh.before_m = m;
-            sh.found_m = m + sh.w[digit & 255];
-            sh.n = digit;
-        }
-        __syncthreads();
-        prefix |= static_cast<uint64_t>(sh.n) << shift;
-        base_n = sh.before_n;
-        base_m = sh.before_m;
+        prefix |= static_cast<u64>(sh.digit) << shift;
+        before_n = sh.before_n;
+        before_m = sh.before_m;
     }
-    *upto = sh.found_m;
+    *upto = sh.found_upto;
     return prefix;
 }
 
 template <class T>
-__global__ __launch_bounds__(kThreads) void sample_row_kernel(SampleArgs p) {
-    __shared__ Shared sh;
+__global__ __launch_bounds__(kPick) void sample_pick_kernel(SampleArgs p) {
+    __shared__ PickShared sh;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const T* row = static_cast<const T*>(p.logits) + blockIdx.x * p.ld;
-    const int V = p.V;
-    // the maximum, at its lowest index
-    uint64_t best = ~0ull;
-    for (int i = tid; i < V; i += kThreads) best = min(best, order_key(logit(row, i), i));
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) best = min(best, static_cast<uint64_t>(__shfl_xor(static_cast<u64>(best), o, 64)));
-    if (lane == 0) sh.best[wave] = best;
-    __syncthreads();
-    for (int w = 0; w < kThreads / 64; ++w) best = min(best, sh.best[w]);
-    const float t = p.temperature ? p.temperature[blockIdx.x] : 1.f;
-    Row r;
-    r.M = key_value(best);
-    if (r.M == -INFINITY || !(t > 0.f)) {
+    const size_t row = blockIdx.x;
+    const T* zr = static_cast<const T*>(p.logits) + row * p.ld;
+    const Row r = settings(p, row, row_max(p, row, sh.fpart));
+    if (r.greedy) {
+        // the first chunk with the maximum, its first such logit
+        if (tid == 0) sh.at = p.chunks, sh.n = p.V;
+        __syncthreads();
+        for (int c = tid; c < p.chunks; c += kPick)
+            if (p.cmax[row * p.chunks + c] == r.M) atomicMin(&sh.at, c);
+        __syncthreads();
+        const int begin = sh.at * p.chunk, end = min(p.V, begin + p.chunk);
+        for (int i = begin + tid; i < end; i += kPick)
+            if (clean(static_cast<float>(zr[i])) == r.M) {
+                atomicMin(&sh.n, i);
+                break;
+            }
+        __syncthreads();
         if (tid == 0) {
-            p.idx[blockIdx.x] = r.M == -INFINITY ? 0 : static_cast<int>(best & 0xffffffffu);
-            if (p.prob) p.prob[blockIdx.x] = r.M == -INFINITY ? 0.f : 1.f;
+            p.idx[row] = r.M == -INFINITY ? 0 : sh.n;
+            if (p.prob) p.prob[row] = r.M == -INFINITY ? 0.f : 1.f;
         }
         return;
     }
-    r.inv_t = 1.0 / static_cast<double>(t);
-    r.unit = ldexp(1.0, p.shift);
-    const float mp = p.min_p ? p.min_p[blockIdx.x] : 0.f;
-    r.min_p = mp > 0.f ? fminf(mp, 1.f) : 0.0;
-    const int k = p.top_k ? p.top_k[blockIdx.x] : 0;
-    const float tp = p.top_p ? p.top_p[blockIdx.x] : 1.f;
-    const bool use_k = k > 0 && k < V, use_p = tp < 1.f;
-    uint64_t last = ~0ull;
-    if (use_k || use_p) {
-        for (int i = tid; i < kBins; i += kThreads) {
-            sh.cnt[i] = 0;
-            sh.mass[i] = 0;
-        }
+    // shares of whole tiles, one per thread
+    const int per = (p.tiles + kPick - 1) / kPick, share = per * kTile;
+    u64 last = ~0ull;
+    bool listed = true;  // the tiles' masses and the list hold everything
+    int n_list = 0;
+    Borders b{kBins, kBins, kBins, 0, 0, 0};
+    if (r.filters()) {
+        b = borders<kPick>(p, row, r, sh.b);
+        const unsigned n = p.cnt[row * (kBins + 1) + kBins];
+        listed = n <= kList;
+        n_list = listed ? n : 0;
+        for (int i = tid; i < n_list; i += kPick) sh.key[i] = p.list[row * kList + i];
         __syncthreads();
-        for (int i = tid; i < V; i += kThreads) {
-            const double d = r.depth(logit(row, i));
-            if (d >= 32.0) continue;
-            const u64 m = r.mass(r.weight(d));
-            if (m == 0) continue;
-            atomicAdd(&sh.cnt[r.bin(d)], 1u);
-            atomicAdd(&sh.mass[r.bin(d)], m);
-        }
-        __syncthreads();
-        unsigned c[2], ci;
-        u64 m[2], mi;
-        for (int e = 0; e < 2; ++e) {
-            c[e] = sh.cnt[2 * tid + e];
-            m[e] = sh.mass[2 * tid + e];
-        }
-        ci = block_scan(c[0] + c[1], sh.cpart);
-        mi = block_scan(m[0] + m[1], sh.part);
-        unsigned total_n = 0;
-        u64 total_m = 0;
-        for (int w = 0; w < kThreads / 64; ++w) {
-            total_n += sh.cpart[w];
-            total_m += sh.part[w];
-        }
-        int k_bin = kBins;
-        if (use_k && static_cast<unsigned>(k) < total_n) {
-            unsigned b0 = ci - c[0] - c[1];
-            u64 m0 = mi - m[0] - m[1];
-            for (int e = 0; e < 2; ++e) {
-                if (b0 < static_cast<unsigned>(k) && static_cast<unsigned>(k) <= b0 + c[e]) {
-                    sh.bin = 2 * tid + e;
-                    sh.before_n = b0;
-                    sh.before_m = m0;
+        const auto each_of = [&](int bin_lo, int bin_hi, u64 upto, auto f) {
+            if (listed) {
+                for (int i = tid; i < n_list; i += kPick) {
+                    const u64 key = sh.key[i];
+                    const double d = r.depth(key_value(key));
+                    if (r.bin(d) >= bin_lo && r.bin(d) <= bin_hi && key <= upto) f(key, r.mass(d));
                 }
-                b0 += c[e];
-                m0 += m[e];
-            }
-            __syncthreads();
-            k_bin = sh.bin;
-            last = find_in_bin(p, row, r, sh, last, k, 0.0, &total_m);
-            __syncthreads();
-        }
-        if (use_p) {
-            const double want = fmax(static_cast<double>(tp) * static_cast<double>(total_m), 0.5);
-            u64 m0 = mi - m[0] - m[1];
-            for (int e = 0; e < 2; ++e) {
-                // what top-k cut off the last bin, and the bins behind it, do not count
-                const u64 m1 = 2 * tid + e < k_bin ? m0 + m[e] : total_m;
-                if (2 * tid + e <= k_bin && static_cast<double>(m0) < want && static_cast<double>(m1) >= want) {
-                    sh.bin = 2 * tid + e;
-                    sh.before_n = 0;
-                    sh.before_m = m0;
+            } else {
+                const float low = r.below(fmin((bin_hi + 1) / kBinsPerUnit, kDepth));
+                for (int i = tid; i < p.V; i += kPick) {
+                    const float z = clean(static_cast<float>(zr[i]));
+                    if (!(z >= low)) continue;
+                    const double d = r.depth(z);
+                    if (d >= kDepth || r.bin(d) < bin_lo || r.bin(d) > bin_hi) continue;
+                    const u64 key = order_key(z, i);
+                    if (key <= upto) f(key, r.mass(d));
                 }
-                m0 += m[e];
             }
-            __syncthreads();
+        };
+        u64 left = b.all;
+        if (b.k_bin < kBins)
+            last = find_last(sh, [&](auto f) { each_of(b.k_bin, b.k_bin, ~0ull, f); }, b.k_before, b.k_mass, r.top_k, 0.0, &left);
+        if (r.use_p) {
+            // the bins from b.sure on hold the border; the mass before them
+            const double want = fmax(r.top_p * static_cast<double>(left), 0.5);
+            u64 m = 0;
+            for (int i = tid; i < b.sure; i += kPick) m += p.mass[row * kBins + i];
+            u64 before;
+            block_scan(m, sh.part, &before);
             u64 upto;
-            last = find_in_bin(p, row, r, sh, last, 0, want, &upto);
+            last = find_last(sh, [&](auto f) { each_of(b.sure, b.top, last, f); }, 0, before, 0, want, &upto);
         }
         __syncthreads();
     }
-    // mass by blocks of the row, then the block the number falls in
+    sh.range[tid] = 0;
+    __syncthreads();
     const auto kept = [&](int i) -> u64 {
-        const float z = logit(row, i);
-        const double d = r.depth(z);
-        if (d >= 32.0 || order_key(z, i) > last) return 0;
-        const double w = r.weight(d);
-        return w >= r.min_p ? r.mass(w) : 0;
+        const float z = clean(static_cast<float>(zr[i]));
+        return order_key(z, i) <= last ? r.kept(r.depth(z)) : 0;
     };
-    const int bs = ((V + kThreads - 1) / kThreads + 63) / 64 * 64;
-    u64* blk = sh.mass;
-    for (int b = wave; b < kThreads; b += kThreads / 64) {
+    if (listed) {
         u64 m = 0;
-        for (int i = b * bs + lane; i < min(V, (b + 1) * bs); i += 64) m += kept(i);
-#pragma unroll
-        for (int o = 32; o > 0; o >>= 1) m += __shfl_xor(m, o, 64);
-        if (lane == 0) blk[b] = m;
+        for (int t = tid * per; t < min(p.tiles, (tid + 1) * per); ++t) m += p.tmass[row * p.tiles + t];
+        sh.range[tid] = m;
+        __syncthreads();
+        for (int i = tid; i < n_list; i += kPick) {
+            const u64 key = sh.key[i];
+            if (key <= last) atomicAdd(&sh.range[static_cast<uint32_t>(key) / share], r.kept(r.depth(key_value(key))));
+        }
+    } else {
+        for (int t = wave; t < p.tiles; t += kPick / 64) {
+            u64 m = 0;
+            for (int i = t * kTile + lane; i < min(p.V, (t + 1) * kTile); i += 64) m += kept(i);
+            m = wave_sum64(m);
+            if (lane == 0) atomicAdd(&sh.range[t / per], m);
+        }
     }
     __syncthreads();
-    const u64 mine = blk[tid], upto = block_scan(mine, sh.part);
-    u64 total = 0;
-    for (int w = 0; w < kThreads / 64; ++w) total += sh.part[w];
-    const float u0 = p.u[blockIdx.x];
+    const u64 mine = sh.range[tid];
+    u64 total;
+    const u64 upto = block_scan(mine, sh.part, &total);
+    const float u0 = p.u[row];
     const double target = static_cast<double>(u0 >= 0.f ? fminf(u0, 0.99999994f) : 0.f) * static_cast<double>(total);
     if (mine && static_cast<double>(upto - mine) <= target && static_cast<double>(upto) > target) {
-        sh.bin = tid;
+        sh.at = tid;
         sh.before_m = upto - mine;
     }
     __syncthreads();
-    const int b = sh.bin;
-    u64 before = sh.before_m;
-    for (int i0 = b * bs; i0 < min(V, (b + 1) * bs); i0 += kThreads) {
-        const int i = i0 + tid;
-        const u64 m = i < min(V, (b + 1) * bs) ? kept(i) : 0;
-        const u64 at = before + block_scan(m, sh.part);
-        if (m && static_cast<double>(at - m) <= target && static_cast<double>(at) > target) {
-            p.idx[blockIdx.x] = i;
-            if (p.prob) p.prob[blockIdx.x] = static_cast<float>(static_cast<double>(m) / static_cast<double>(total));
+    // the share's logits, a run of them per thread
+    const int begin = sh.at * share, run = (share + kPick - 1) / kPick;
+    const int i0 = begin + tid * run, i1 = min(p.V, min(begin + share, i0 + run));
+    u64 m = 0;
+    for (int i = i0; i < i1; ++i) m += kept(i);
+    const u64 before = sh.before_m;
+    u64 at = block_scan(m, sh.part) + before - m;
+    if (m && static_cast<double>(at) <= target && static_cast<double>(at + m) > target) {
+        for (int i = i0; i < i1; ++i) {
+            const u64 w = kept(i);
+            at += w;
+            if (w && static_cast<double>(at) > target) {
+                p.idx[row] = i;
+                if (p.prob) p.prob[row] = static_cast<float>(static_cast<double>(w) / static_cast<double>(total));
+                break;
+            }
         }
-        for (int w = 0; w < kThreads / 64; ++w) before += sh.part[w];
     }
 }
 
+// Logits of a workgroup: about 1024 workgroups for all rows, whole rounds of 256 threads x 8.
+int chunk_of(int rows, int V) {
+    const int64_t want = static_cast<int64_t>(rows) * V / 1024;
+    return static_cast<int>(std::max<int64_t>((want + 2047) / 2048, V / 512 / 2048 + 1)) * 2048;
+}
+struct SampleSpace {
+    size_t cmax, cnt, mass, tmass, list, bytes;
+};
+SampleSpace sample_space(int rows, int V, int chunks, int tiles) {
+    SampleSpace s;
+    const size_t n = rows;
+    s.mass = 0;
+    s.tmass = s.mass + n * kBins * 8;
+    s.list = s.tmass + n * tiles * 8;
+    s.cnt = s.list + n * kList * 8;
+    s.cmax = s.cnt + n * (kBins + 1) * 4;
+    s.bytes = (s.cmax + n * chunks * 4 + 255) / 256 * 256;
+    return s;
+}
+
 size_t sample_workspace_bytes(int rows, int V) {
-    (void)rows, (void)V;
-    return 256;
+    if (rows < 1 || V < 1) return 256;
+    const int chunk = chunk_of(rows, V);
+    return sample_space(rows, V, (V + chunk - 1) / chunk, (V + kTile - 1) / kTile).bytes;
+}
+
+template <class T>
+void launch_sample(const SampleArgs& p, int rows, hipStream_t s) {
+    const dim3 grid(rows * p.chunks);
+    hipLaunchKernelGGL(sample_max_kernel<T>, grid, dim3(256), 0, s, p);
+    check_launch("sample_max_kernel");
+    hipLaunchKernelGGL(sample_hist_kernel<T>, grid, dim3(256), 0, s, p);
+    check_launch("sample_hist_kernel");
+    if (p.top_k || p.top_p) {
+        hipLaunchKernelGGL(sample_list_kernel<T>, grid, dim3(256), 0, s, p);
+        check_launch("sample_list_kernel");
+    }
+    hipLaunchKernelGGL(sample_pick_kernel<T>, dim3(rows), dim3(kPick), 0, s, p);
+    check_launch("sample_pick_kernel");
 }
 
 void sample_rows(int dtype, const void* logits, int64_t ld, int rows, int V, const float* temperature, const int* top_k,
@@ -344,7 +606,7 @@ void sample_rows(int dtype, const void* logits, int64_t ld, int rows, int V, con
                  hipStream_t s) {
     RL_REQUIRE(dtype == RL_Q_F32 || dtype == RL_Q_F16 || dtype == RL_Q_BF16, RL_ERR_UNSUPPORTED,
                "sample_rows: logits must be F32, F16 or BF16");
-    RL_REQUIRE(rows >= 0 && V >= 1 && V <= 1 << 24 && ld >= V, RL_ERR_RANGE, "sample_rows: bad sizes");
+    RL_REQUIRE(rows >= 0 && rows <= 1 << 20 && V >= 1 && V <= 1 << 24 && ld >= V, RL_ERR_RANGE, "sample_rows: bad sizes");
     if (rows == 0) return;
     RL_REQUIRE(logits && u && idx && ws, RL_ERR_RANGE, "sample_rows: null pointer");
     RL_REQUIRE(aligned(logits, type_bytes(dtype)) && aligned(ws, 16), RL_ERR_RANGE, "sample_rows: misaligned pointer");
@@ -354,15 +616,25 @@ void sample_rows(int dtype, const void* logits, int64_t ld, int rows, int V, con
     int bits = 0;
     while ((1 << bits) < V) ++bits;
     p.shift = std::min(44, 62 - bits);
+    p.chunk = chunk_of(rows, V);
+    p.chunks = (V + p.chunk - 1) / p.chunk;
+    p.tiles = (V + kTile - 1) / kTile;
+    p.wide = aligned(logits, 16) && ld * type_bytes(dtype) % 16 == 0;
     p.temperature = temperature, p.top_k = top_k, p.top_p = top_p, p.min_p = min_p, p.u = u;
     p.idx = idx, p.prob = prob;
+    const SampleSpace sp = sample_space(rows, V, p.chunks, p.tiles);
+    char* w = static_cast<char*>(ws);
+    p.mass = reinterpret_cast<u64*>(w + sp.mass);
+    p.tmass = reinterpret_cast<u64*>(w + sp.tmass);
+    p.list = reinterpret_cast<u64*>(w + sp.list);
+    p.cnt = reinterpret_cast<unsigned*>(w + sp.cnt);
+    p.cmax = reinterpret_cast<float*>(w + sp.cmax);
     if (dtype == RL_Q_F32)
-        hipLaunchKernelGGL(sample_row_kernel<float>, dim3(rows), dim3(kThreads), 0, s, p);
+        launch_sample<float>(p, rows, s);
     else if (dtype == RL_Q_F16)
-        hipLaunchKernelGGL(sample_row_kernel<_Float16>, dim3(rows), dim3(kThreads), 0, s, p);
+        launch_sample<_Float16>(p, rows, s);
     else
-        hipLaunchKernelGGL(sample_row_kernel<__bf16>, dim3(rows), dim3(kThreads), 0, s, p);
-    check_launch("sample_row_kernel");
+        launch_sample<__bf16>(p, rows, s);
 }
 
 }  // namespace
