@@ -8,10 +8,12 @@
 // follows from the masses of tiles of 512 logits, then from one tile's logits.
 // Masses are integers (w in units of 2^-44 of the largest), so that sums are exact in any order and
 // every kernel sees the same element the same way.
-// Four launches, the first three with many workgroups per row: maximum; histogram (rows without
-// top-k and top-p: the tiles' masses already); the tiles' surely kept masses and a list of the
-// border bins' elements (such rows skip it); the choice.  One workgroup per row doing all of it took
-// 344 us for one row of 248320 logits, 633 us for 128.
+// Four launches, the first three with many workgroups per row: maxima of the tiles; a histogram (rows
+// without top-k and top-p: the tiles' masses already); the tiles' surely kept masses and a list of the
+// border bins' elements; the choice.  Up to kSmallK, all that top-k may keep goes to the list and the
+// histogram needs no masses; where there are 2 k tiles (or groups of them) it is not needed at all: the k-th
+// largest of their maxima is a bound that at least k elements reach, and few others do.  One workgroup per row
+// doing all of it took 344 us for one row of 248320 logits, 633 us for 128.
 #include <algorithm>
 #include <cmath>
 
@@ -28,6 +30,9 @@ constexpr int kBins = 2048;
 constexpr double kBinsPerUnit = 44.0;  // bins of depth
 constexpr double kDepth = 45.0;        // weights from 2^-45 down are no unit
 constexpr int kList = 4096;            // elements of the border bins that are listed
+constexpr int kSmallK = 2048;
+constexpr int kBound = 512;            // maxima that a wave finds the k-th largest of
+constexpr int kRanked = 1024;          // elements that are put in order by counting the ones before each
 constexpr int kPick = 1024;            // threads of the last launch
 
 struct SampleArgs {
@@ -35,12 +40,14 @@ struct SampleArgs {
     int64_t ld;
     int V, shift;  // masses in units of 2^-shift
     int chunk, chunks, tiles;  // logits of a workgroup, workgroups and tiles of a row
+    int group, groups;         // tiles of a group, groups of a row: up to kBound
     const float *temperature, *top_p, *min_p, *u;
     const int* top_k;
     int* idx;
     float* prob;
     // workspace, per row
     float* cmax;   // [chunks]
+    float* tmax;   // [tiles]
     unsigned* cnt; // [kBins] + the list's length
     u64* mass;     // [kBins]
     u64* tmass;    // [tiles]
@@ -106,6 +113,9 @@ struct Row {
     int shift, top_k;  // 0: off
     bool greedy, use_p;
     __device__ bool filters() const { return top_k || use_p; }
+    __device__ bool small_k() const { return top_k && top_k <= kSmallK; }
+    __device__ bool bounded(const SampleArgs& p) const { return top_k && top_k <= p.groups / 2; }
+    __device__ bool masses() const { return use_p && !small_k(); }  // in the histogram
     // (M - z) / (T ln 2), >= 0; past kDepth for what has no weight at all
     __device__ double depth(float z) const {
         if (z == M) return 0.0;
@@ -154,10 +164,10 @@ __device__ inline Row settings(const SampleArgs& p, int row, float M) {
     return r;
 }
 
-// Sum over the waves before, and of all; every thread calls it.  part: one per wave.
-template <class T>
+// Inclusive sum over the workgroup's kThreads threads, and all of it; every thread calls it.
+template <int kThreads, class T>
 __device__ inline T block_scan(T v, T* part, T* total = nullptr) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
         const T x = __shfl_up(v, o, 64);
@@ -167,9 +177,11 @@ __device__ inline T block_scan(T v, T* part, T* total = nullptr) {
     if (lane == 63) part[wave] = v;
     __syncthreads();
     T before = 0, all = 0;
-    for (int w = 0; w < waves; ++w) {
-        if (w < wave) before += part[w];
-        all += part[w];
+#pragma unroll
+    for (int w = 0; w < kThreads / 64; ++w) {
+        const T x = part[w];
+        before += w < wave ? x : 0;
+        all += x;
     }
     if (total) *total = all;
     return v + before;
@@ -206,12 +218,17 @@ template <class T>
 __global__ __launch_bounds__(256) void sample_max_kernel(SampleArgs p) {
     __shared__ float part_s[4];
     const Part<T> a = part_of<T>(p);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     float m = -INFINITY;
-    for (int i = a.begin + 8 * threadIdx.x; i < a.end; i += 8 * 256) {
+    for (int t = a.begin / kTile + wave; t * kTile < a.end; t += 4) {
         float z[8];
-        load8(a.z, i, a.end, p.wide, z);
+        load8(a.z, t * kTile + 8 * lane, a.end, p.wide, z);
+        float x = z[0];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) m = fmaxf(m, z[e]);
+        for (int e = 1; e < 8; ++e) x = fmaxf(x, z[e]);
+        x = wave_max(x);
+        m = fmaxf(m, x);
+        if (lane == 0) p.tmax[static_cast<size_t>(a.row) * p.tiles + t] = x;
     }
     m = block_max(m, part_s);
     if (threadIdx.x == 0) p.cmax[static_cast<size_t>(a.row) * p.chunks + a.chunk] = m;
@@ -236,7 +253,7 @@ __global__ __launch_bounds__(256) void sample_hist_kernel(SampleArgs p) {
     __shared__ u64 mass_s[kBins];
     const Part<T> a = part_of<T>(p);
     const Row r = settings(p, a.row, row_max(p, a.row, part_s));
-    if (r.greedy) return;
+    if (r.greedy || r.bounded(p)) return;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const float low = r.below(kDepth);
     if (!r.filters()) {
@@ -252,28 +269,32 @@ __global__ __launch_bounds__(256) void sample_hist_kernel(SampleArgs p) {
         }
         return;
     }
+    const bool masses = r.masses();
     for (int i = threadIdx.x; i < kBins; i += 256) {
         cnt_s[i] = 0;
-        mass_s[i] = 0;
+        if (masses) mass_s[i] = 0;
     }
     __syncthreads();
+    float z[8], next[8];
+    load8(a.z, a.begin + 8 * threadIdx.x, a.end, p.wide, next);
     for (int i = a.begin + 8 * threadIdx.x; i < a.end; i += 8 * 256) {
-        float z[8];
-        load8(a.z, i, a.end, p.wide, z);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) z[e] = next[e];
+        load8(a.z, i + 8 * 256, a.end, p.wide, next);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
             if (!(z[e] >= low)) continue;
             const double d = r.depth(z[e]);
             if (d >= kDepth) continue;
             if (r.top_k) atomicAdd(&cnt_s[r.bin(d)], 1u);
-            if (r.use_p) atomicAdd(&mass_s[r.bin(d)], r.mass(d));
+            if (masses) atomicAdd(&mass_s[r.bin(d)], r.mass(d));
         }
     }
     __syncthreads();
     const size_t row = a.row;
     for (int i = threadIdx.x; i < kBins; i += 256) {
         if (r.top_k && cnt_s[i]) atomicAdd(&p.cnt[row * (kBins + 1) + i], cnt_s[i]);
-        if (r.use_p && mass_s[i]) atomicAdd(&p.mass[row * kBins + i], mass_s[i]);
+        if (masses && mass_s[i]) atomicAdd(&p.mass[row * kBins + i], mass_s[i]);
     }
 }
 
@@ -301,13 +322,13 @@ __device__ Borders borders(const SampleArgs& p, int row_, const Row& r, BorderSh
 #pragma unroll
     for (int e = 0; e < E; ++e) {
         c[e] = r.top_k ? p.cnt[row * (kBins + 1) + tid * E + e] : 0;
-        m[e] = r.use_p ? p.mass[row * kBins + tid * E + e] : 0;
+        m[e] = r.masses() ? p.mass[row * kBins + tid * E + e] : 0;
         cs += c[e];
         ms += m[e];
     }
     if (tid == 0) sh.k_bin = kBins, sh.lo = sh.hi = kBins;
-    const unsigned c0 = block_scan(cs, sh.cpart, &ct) - cs;
-    const u64 m0 = block_scan(ms, sh.part, &mt) - ms;
+    const unsigned c0 = block_scan<kThreads>(cs, sh.cpart, &ct) - cs;
+    const u64 m0 = block_scan<kThreads>(ms, sh.part, &mt) - ms;
     if (r.top_k && static_cast<unsigned>(r.top_k) < ct) {
         unsigned cb = c0;
         u64 mb = m0;
@@ -330,7 +351,9 @@ __device__ Borders borders(const SampleArgs& p, int row_, const Row& r, BorderSh
     b.k_mass = sh.k_mass;
     b.all = mt;
     b.sure = b.top = b.k_bin;
-    if (r.use_p) {
+    if (r.small_k()) {
+        b.sure = 0;  // all of it is listed
+    } else if (r.use_p) {
         // top-k leaves between k_mass and that with all of its last bin
         const u64 least = b.k_bin < kBins ? b.k_mass : mt, most = b.k_bin < kBins ? b.k_mass + sh.k_own : mt;
         const double lo = fmax(r.top_p * static_cast<double>(least), 0.5), hi = fmax(r.top_p * static_cast<double>(most), 0.5);
@@ -349,58 +372,140 @@ __device__ Borders borders(const SampleArgs& p, int row_, const Row& r, BorderSh
     return b;
 }
 
+// The k-th largest of the maxima of groups of tiles: at least k logits reach it.  A wave's work, bit by bit
+// from the top.
+__device__ float kth_max(const SampleArgs& p, int row, int k) {
+    const int lane = threadIdx.x & 63, per = p.group;
+    uint32_t v[kBound / 64];
+#pragma unroll
+    for (int i = 0; i < kBound / 64; ++i) {
+        float m = -INFINITY;
+        const int g = 64 * i + lane;
+        for (int t = g * per; t < min(p.tiles, (g + 1) * per); ++t) m = fmaxf(m, p.tmax[static_cast<size_t>(row) * p.tiles + t]);
+        const uint32_t b = __float_as_uint(m);
+        v[i] = b >> 31 ? ~b : b | 0x80000000u;  // ordered as the values
+    }
+    uint32_t x = 0;
+    for (int bit = 31; bit >= 0; --bit) {
+        const uint32_t y = x | 1u << bit;
+        int n = 0;
+#pragma unroll
+        for (int i = 0; i < kBound / 64; ++i) n += __popcll(__ballot(v[i] >= y));
+        if (n >= k) x = y;
+    }
+    return __uint_as_float(x >> 31 ? x & 0x7fffffffu : ~x);
+}
+
 template <class T>
 __global__ __launch_bounds__(256) void sample_list_kernel(SampleArgs p) {
     __shared__ float part_s[4];
     __shared__ BorderShared sh;
+    __shared__ u64 key_s[kList];
+    __shared__ int n_s, at_s;
     const Part<T> a = part_of<T>(p);
     const Row r = settings(p, a.row, row_max(p, a.row, part_s));
     if (r.greedy || !r.filters()) return;
-    const Borders b = borders<256>(p, a.row, r, sh);
-    const int last = b.k_bin < kBins ? b.k_bin : b.top;  // the last bin looked at
-    const float low = r.below(fmin((last + 1) / kBinsPerUnit, kDepth));
+    Borders b{0, kBins, kBins, 0, 0, 0};
+    float low;
+    if (r.bounded(p)) {
+        low = fmaxf(r.below(kDepth), kth_max(p, a.row, r.top_k));
+    } else {
+        b = borders<256>(p, a.row, r, sh);
+        const int last = b.k_bin < kBins ? b.k_bin : b.top;  // the last bin looked at
+        low = r.below(fmin((last + 1) / kBinsPerUnit, kDepth));
+    }
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const size_t row = a.row;
+    if (threadIdx.x == 0) n_s = 0;
+    __syncthreads();
+    float z[8], next[8];
+    load8(a.z, a.begin + wave * kTile + 8 * lane, a.end, p.wide, next);
     for (int t = a.begin / kTile + wave; t * kTile < a.end; t += 4) {
-        float z[8];
         const int i = t * kTile + 8 * lane;
-        load8(a.z, i, a.end, p.wide, z);
         u64 m = 0;
+        bool any = false;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            if (!(z[e] >= low)) continue;
-            const double d = r.depth(z[e]);
-            if (d >= kDepth) continue;
-            const int bin = r.bin(d);
-            if (bin < b.sure) {
-                m += r.kept(d);
-            } else if (bin <= b.top || bin == b.k_bin) {
-                const unsigned at = atomicAdd(&p.cnt[row * (kBins + 1) + kBins], 1u);
-                if (at < kList) p.list[row * kList + at] = order_key(z[e], i + e);
+            z[e] = next[e];
+            any |= z[e] >= low;
+        }
+        load8(a.z, i + 4 * kTile, a.end, p.wide, next);
+        if (any) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                if (!(z[e] >= low)) continue;
+                const double d = r.depth(z[e]);
+                if (d >= kDepth) continue;
+                const int bin = r.bin(d);
+                if (bin < b.sure) {
+                    m += r.kept(d);
+                } else if (bin <= b.top || bin == b.k_bin) {
+                    const int at = atomicAdd(&n_s, 1);
+                    if (at < kList) key_s[at] = order_key(z[e], i + e);
+                }
             }
         }
+        if (b.sure == 0) continue;  // nothing is kept unseen
         m = wave_sum64(m);
         if (lane == 0) p.tmass[row * p.tiles + t] = m;
     }
+    __syncthreads();
+    if (threadIdx.x == 0 && n_s) at_s = static_cast<int>(atomicAdd(&p.cnt[row * (kBins + 1) + kBins], static_cast<unsigned>(n_s)));
+    __syncthreads();
+    for (int i = threadIdx.x; i < min(n_s, kList) && at_s + i < kList; i += 256) p.list[row * kList + at_s + i] = key_s[i];
 }
 
 struct PickShared {
     BorderShared b;
     float fpart[kPick / 64];
+    unsigned cpart[kPick / 64];
     u64 part[kPick / 64];
-    u64 key[kList];   // the list; where it does not hold the border bins, the radix search's counts
-    u64 range[kPick]; // masses of equal shares of the row
+    u64 key[kList], w[kList];       // the list and its masses
+    unsigned cnt[kBins];
+    u64 mass[kBins];
+    u64 range[kPick];               // masses of equal shares of the row
+    u64 sub[kRanked], sub_w[kRanked];
     u64 dig_n[256], dig_m[256];
     u64 found_key, found_upto, before_m;
     unsigned before_n;
-    int digit, n, at;
+    int digit, n, at, bin;
 };
 
 // Which of the elements that `each` hands out ends the prefix: the one with `want_n` up to it (before_n stand
 // before all of them), or else the first up to which want_m of mass stands.  The key of it, *upto the mass up to it.
 template <class Each>
 __device__ u64 find_last(PickShared& sh, Each each, unsigned before_n, u64 before_m, unsigned want_n, double want_m, u64* upto) {
-    // eight bits of the key at a time
+    __syncthreads();
+    if (threadIdx.x == 0) sh.n = 0;
+    __syncthreads();
+    each([&](u64 key, u64 m) {
+        const int at = atomicAdd(&sh.n, 1);
+        if (at < kRanked) sh.sub[at] = key, sh.sub_w[at] = m;
+    });
+    __syncthreads();
+    const int n_sub = sh.n;
+    if (n_sub <= kRanked) {
+        if (static_cast<int>(threadIdx.x) < n_sub) {
+            const u64 key = sh.sub[threadIdx.x], m = sh.sub_w[threadIdx.x];
+            unsigned n = before_n;
+            u64 before = before_m;
+            for (int j = 0; j < n_sub; ++j) {
+                const bool less = sh.sub[j] < key;
+                n += less;
+                before += less ? sh.sub_w[j] : 0;
+            }
+            const bool hit = want_n ? n + 1 == want_n
+                                    : static_cast<double>(before) < want_m && static_cast<double>(before + m) >= want_m;
+            if (hit) {
+                sh.found_key = key;
+                sh.found_upto = before + m;
+            }
+        }
+        __syncthreads();
+        *upto = sh.found_upto;
+        return sh.found_key;
+    }
+    // many (flat or repeated logits): eight bits of the key at a time
     u64 prefix = 0;
     for (int shift = 56; shift >= 0; shift -= 8) {
         __syncthreads();
@@ -414,7 +519,7 @@ __device__ u64 find_last(PickShared& sh, Each each, unsigned before_n, u64 befor
         __syncthreads();
         u64 n = 0, m = 0;
         if (threadIdx.x < 256) n = sh.dig_n[threadIdx.x], m = sh.dig_m[threadIdx.x];
-        const u64 ni = block_scan(n, sh.part) + before_n, mi = block_scan(m, sh.part) + before_m;
+        const u64 ni = block_scan<kPick>(n, sh.part) + before_n, mi = block_scan<kPick>(m, sh.part) + before_m;
         const bool hit = want_n ? ni - n < want_n && want_n <= ni
                                 : static_cast<double>(mi - m) < want_m && static_cast<double>(mi) >= want_m;
         if (n && hit) {
@@ -464,20 +569,22 @@ __global__ __launch_bounds__(kPick) void sample_pick_kernel(SampleArgs p) {
     u64 last = ~0ull;
     bool listed = true;  // the tiles' masses and the list hold everything
     int n_list = 0;
-    Borders b{kBins, kBins, kBins, 0, 0, 0};
+    int sure = kBins;  // bins before it are in the tiles' masses
     if (r.filters()) {
-        b = borders<kPick>(p, row, r, sh.b);
         const unsigned n = p.cnt[row * (kBins + 1) + kBins];
         listed = n <= kList;
         n_list = listed ? n : 0;
-        for (int i = tid; i < n_list; i += kPick) sh.key[i] = p.list[row * kList + i];
-        __syncthreads();
+        for (int i = tid; i < n_list; i += kPick) {
+            sh.key[i] = p.list[row * kList + i];
+            sh.w[i] = r.mass(r.depth(key_value(sh.key[i])));
+        }
+        // the elements of some bins with keys up to one: from the list, or where that is too short from the row
         const auto each_of = [&](int bin_lo, int bin_hi, u64 upto, auto f) {
             if (listed) {
                 for (int i = tid; i < n_list; i += kPick) {
                     const u64 key = sh.key[i];
-                    const double d = r.depth(key_value(key));
-                    if (r.bin(d) >= bin_lo && r.bin(d) <= bin_hi && key <= upto) f(key, r.mass(d));
+                    const int bin = r.bin(r.depth(key_value(key)));
+                    if (bin >= bin_lo && bin <= bin_hi && key <= upto) f(key, sh.w[i]);
                 }
             } else {
                 const float low = r.below(fmin((bin_hi + 1) / kBinsPerUnit, kDepth));
@@ -491,18 +598,80 @@ __global__ __launch_bounds__(kPick) void sample_pick_kernel(SampleArgs p) {
                 }
             }
         };
-        u64 left = b.all;
-        if (b.k_bin < kBins)
-            last = find_last(sh, [&](auto f) { each_of(b.k_bin, b.k_bin, ~0ull, f); }, b.k_before, b.k_mass, r.top_k, 0.0, &left);
-        if (r.use_p) {
-            // the bins from b.sure on hold the border; the mass before them
-            const double want = fmax(r.top_p * static_cast<double>(left), 0.5);
-            u64 m = 0;
-            for (int i = tid; i < b.sure; i += kPick) m += p.mass[row * kBins + i];
-            u64 before;
-            block_scan(m, sh.part, &before);
-            u64 upto;
-            last = find_last(sh, [&](auto f) { each_of(b.sure, b.top, last, f); }, 0, before, 0, want, &upto);
+        if (r.small_k()) {
+            // a histogram of the list, top-k's border in it, then top-p's in what that leaves
+            sure = 0;
+            for (int i = tid; i < kBins; i += kPick) sh.cnt[i] = 0, sh.mass[i] = 0;
+            if (tid == 0) sh.bin = kBins;
+            __syncthreads();
+            each_of(0, kBins, ~0ull, [&](u64 key, u64 m) {
+                const int bin = r.bin(r.depth(key_value(key)));
+                atomicAdd(&sh.cnt[bin], 1u);
+                atomicAdd(&sh.mass[bin], m);
+            });
+            __syncthreads();
+            constexpr int E = kBins / kPick;
+            unsigned c[E], cs = 0, ct;
+            u64 m[E], ms = 0, left;
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                cs += c[e] = sh.cnt[tid * E + e];
+                ms += m[e] = sh.mass[tid * E + e];
+            }
+            const unsigned c0 = block_scan<kPick>(cs, sh.cpart, &ct) - cs;
+            const u64 m0 = block_scan<kPick>(ms, sh.part, &left) - ms;
+            int k_bin = kBins;
+            if (static_cast<unsigned>(r.top_k) <= ct) {  // fewer: the list has all that weighs anything
+                unsigned cb = c0;
+                u64 mb = m0;
+#pragma unroll
+                for (int e = 0; e < E; ++e) {
+                    if (cb < static_cast<unsigned>(r.top_k) && static_cast<unsigned>(r.top_k) <= cb + c[e]) {
+                        sh.bin = tid * E + e;
+                        sh.before_n = cb;
+                        sh.before_m = mb;
+                    }
+                    cb += c[e];
+                    mb += m[e];
+                }
+                __syncthreads();
+                k_bin = sh.bin;
+                last = find_last(sh, [&](auto f) { each_of(k_bin, k_bin, ~0ull, f); }, sh.before_n, sh.before_m, r.top_k, 0.0, &left);
+            }
+            if (r.use_p) {
+                const double want = fmax(r.top_p * static_cast<double>(left), 0.5);
+                __syncthreads();
+                u64 mb = m0;
+#pragma unroll
+                for (int e = 0; e < E; ++e) {
+                    const int bin = tid * E + e;
+                    const u64 me = bin < k_bin ? mb + m[e] : left;
+                    if (bin <= k_bin && static_cast<double>(mb) < want && static_cast<double>(me) >= want) {
+                        sh.bin = bin;
+                        sh.before_m = mb;
+                    }
+                    mb += m[e];
+                }
+                __syncthreads();
+                const int p_bin = sh.bin;
+                u64 upto;
+                last = find_last(sh, [&](auto f) { each_of(p_bin, p_bin, last, f); }, 0, sh.before_m, 0, want, &upto);
+            }
+        } else {
+            const Borders b = borders<kPick>(p, row, r, sh.b);
+            sure = b.sure;
+            u64 left = b.all, before = 0;
+            if (b.k_bin < kBins)
+                last = find_last(sh, [&](auto f) { each_of(b.k_bin, b.k_bin, ~0ull, f); }, b.k_before, b.k_mass, r.top_k, 0.0, &left);
+            if (r.use_p) {
+                // the bins from b.sure to b.top hold the border; the mass before them
+                const double want = fmax(r.top_p * static_cast<double>(left), 0.5);
+                u64 m = 0;
+                for (int i = tid; i < b.sure; i += kPick) m += p.mass[row * kBins + i];
+                block_scan<kPick>(m, sh.part, &before);
+                u64 upto;
+                last = find_last(sh, [&](auto f) { each_of(b.sure, b.top, last, f); }, 0, before, 0, want, &upto);
+            }
         }
         __syncthreads();
     }
@@ -514,7 +683,8 @@ __global__ __launch_bounds__(kPick) void sample_pick_kernel(SampleArgs p) {
     };
     if (listed) {
         u64 m = 0;
-        for (int t = tid * per; t < min(p.tiles, (tid + 1) * per); ++t) m += p.tmass[row * p.tiles + t];
+        if (sure > 0)
+            for (int t = tid * per; t < min(p.tiles, (tid + 1) * per); ++t) m += p.tmass[row * p.tiles + t];
         sh.range[tid] = m;
         __syncthreads();
         for (int i = tid; i < n_list; i += kPick) {
@@ -532,7 +702,7 @@ __global__ __launch_bounds__(kPick) void sample_pick_kernel(SampleArgs p) {
     __syncthreads();
     const u64 mine = sh.range[tid];
     u64 total;
-    const u64 upto = block_scan(mine, sh.part, &total);
+    const u64 upto = block_scan<kPick>(mine, sh.part, &total);
     const float u0 = p.u[row];
     const double target = static_cast<double>(u0 >= 0.f ? fminf(u0, 0.99999994f) : 0.f) * static_cast<double>(total);
     if (mine && static_cast<double>(upto - mine) <= target && static_cast<double>(upto) > target) {
@@ -546,7 +716,7 @@ __global__ __launch_bounds__(kPick) void sample_pick_kernel(SampleArgs p) {
     u64 m = 0;
     for (int i = i0; i < i1; ++i) m += kept(i);
     const u64 before = sh.before_m;
-    u64 at = block_scan(m, sh.part) + before - m;
+    u64 at = block_scan<kPick>(m, sh.part) + before - m;
     if (m && static_cast<double>(at) <= target && static_cast<double>(at + m) > target) {
         for (int i = i0; i < i1; ++i) {
             const u64 w = kept(i);
@@ -566,7 +736,7 @@ int chunk_of(int rows, int V) {
     return static_cast<int>(std::max<int64_t>((want + 2047) / 2048, V / 512 / 2048 + 1)) * 2048;
 }
 struct SampleSpace {
-    size_t cmax, cnt, mass, tmass, list, bytes;
+    size_t cmax, tmax, cnt, mass, tmass, list, bytes;
 };
 SampleSpace sample_space(int rows, int V, int chunks, int tiles) {
     SampleSpace s;
@@ -576,7 +746,8 @@ SampleSpace sample_space(int rows, int V, int chunks, int tiles) {
     s.list = s.tmass + n * tiles * 8;
     s.cnt = s.list + n * kList * 8;
     s.cmax = s.cnt + n * (kBins + 1) * 4;
-    s.bytes = (s.cmax + n * chunks * 4 + 255) / 256 * 256;
+    s.tmax = s.cmax + n * chunks * 4;
+    s.bytes = (s.tmax + n * tiles * 4 + 255) / 256 * 256;
     return s;
 }
 
@@ -619,6 +790,8 @@ void sample_rows(int dtype, const void* logits, int64_t ld, int rows, int V, con
     p.chunk = chunk_of(rows, V);
     p.chunks = (V + p.chunk - 1) / p.chunk;
     p.tiles = (V + kTile - 1) / kTile;
+    p.group = (p.tiles + kBound - 1) / kBound;
+    p.groups = (p.tiles + p.group - 1) / p.group;
     p.wide = aligned(logits, 16) && ld * type_bytes(dtype) % 16 == 0;
     p.temperature = temperature, p.top_k = top_k, p.top_p = top_p, p.min_p = min_p, p.u = u;
     p.idx = idx, p.prob = prob;
@@ -629,6 +802,7 @@ void sample_rows(int dtype, const void* logits, int64_t ld, int rows, int V, con
     p.list = reinterpret_cast<u64*>(w + sp.list);
     p.cnt = reinterpret_cast<unsigned*>(w + sp.cnt);
     p.cmax = reinterpret_cast<float*>(w + sp.cmax);
+    p.tmax = reinterpret_cast<float*>(w + sp.tmax);
     if (dtype == RL_Q_F32)
         launch_sample<float>(p, rows, s);
     else if (dtype == RL_Q_F16)
