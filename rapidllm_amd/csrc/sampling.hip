@@ -30,9 +30,11 @@ constexpr int kBins = 2048;
 constexpr double kBinsPerUnit = 44.0;  // bins of depth
 constexpr double kDepth = 45.0;        // weights from 2^-45 down are no unit
 constexpr int kList = 4096;            // elements of the border bins that are listed
+constexpr float kLowest = -3.40282347e38f;
 constexpr int kSmallK = 2048;
 constexpr int kBound = 512;            // maxima that a wave finds the k-th largest of
-constexpr int kRanked = 1024;          // elements that are put in order by counting the ones before each
+constexpr int kRanked = 1024;          // elements that are sorted in shared memory
+constexpr int kCounted = 128;          // ... that are put in order by counting the ones before each
 constexpr int kPick = 1024;            // threads of the last launch
 
 struct SampleArgs {
@@ -48,6 +50,7 @@ struct SampleArgs {
     // workspace, per row
     float* cmax;   // [chunks]
     float* tmax;   // [tiles]
+    float* bound;  // [1] at least top_k logits reach it
     unsigned* cnt; // [kBins] + the list's length
     u64* mass;     // [kBins]
     u64* tmass;    // [tiles]
@@ -122,11 +125,11 @@ struct Row {
         if (z == -INFINITY || M == INFINITY) return 1e9;
         return (static_cast<double>(M) - static_cast<double>(z)) * scale;
     }
-    // everything below has a depth past kDepth, or past the bin's end (one step of z below, for the rounding)
+    // everything below it lies deeper (two steps of z down, for the rounding); never -infinity
     __device__ float below(double depth) const {
         if (M == INFINITY) return M;
         const double z = static_cast<double>(M) - depth / scale;
-        return scale > 0.0 && z > -3e38 ? nextafterf(nextafterf(static_cast<float>(z), -INFINITY), -INFINITY) : -INFINITY;
+        return scale > 0.0 && z > -3e38 ? nextafterf(nextafterf(static_cast<float>(z), -INFINITY), -INFINITY) : kLowest;
     }
     __device__ double weight(double depth) const {
         const double n = rint(depth);
@@ -144,7 +147,13 @@ struct Row {
         const double w = weight(depth);
         return w >= min_p ? mass_of(w) : 0;
     }
-    __device__ static int bin(double depth) { return static_cast<int>(depth * kBinsPerUnit); }
+    // the same without a branch
+    __device__ u64 kept_any(double depth) const {
+        const double w = weight(fmin(depth, kDepth));
+        const u64 m = mass_of(w);
+        return depth < kDepth && w >= min_p ? m : 0;
+    }
+    __device__ static int bin(double depth) { return static_cast<int>(fmin(depth, kDepth) * kBinsPerUnit); }
 };
 
 __device__ inline Row settings(const SampleArgs& p, int row, float M) {
@@ -246,14 +255,46 @@ __device__ inline u64 wave_sum64(u64 v) {
     return v;
 }
 
+// The k-th largest of the maxima of groups of tiles, or a little less: at least k logits reach it.  A wave's
+// work, bit by bit from the top; 11 bits behind the exponent's are enough.
+__device__ float kth_max(const SampleArgs& p, int row, int k) {
+    const int lane = threadIdx.x & 63, per = p.group;
+    uint32_t v[kBound / 64];
+#pragma unroll
+    for (int i = 0; i < kBound / 64; ++i) {
+        float m = -INFINITY;
+        const int g = 64 * i + lane;
+        for (int t = g * per; t < min(p.tiles, (g + 1) * per); ++t) m = fmaxf(m, p.tmax[static_cast<size_t>(row) * p.tiles + t]);
+        const uint32_t b = __float_as_uint(m);
+        v[i] = b >> 31 ? ~b : b | 0x80000000u;  // ordered as the values
+    }
+    uint32_t x = 0;
+    for (int bit = 31; bit >= 12; --bit) {
+        const uint32_t y = x | 1u << bit;
+        int n = 0;
+#pragma unroll
+        for (int i = 0; i < kBound / 64; ++i) n += __popcll(__ballot(v[i] >= y));
+        if (n >= k) x = y;
+    }
+    return __uint_as_float(x >> 31 ? x & 0x7fffffffu : ~x);
+}
+
 template <class T>
 __global__ __launch_bounds__(256) void sample_hist_kernel(SampleArgs p) {
     __shared__ float part_s[4];
     __shared__ unsigned cnt_s[kBins];
     __shared__ u64 mass_s[kBins];
     const Part<T> a = part_of<T>(p);
-    const Row r = settings(p, a.row, row_max(p, a.row, part_s));
-    if (r.greedy || r.bounded(p)) return;
+    Row r = settings(p, a.row, 0.f);
+    if (r.bounded(p)) {
+        if (a.chunk == 0 && threadIdx.x < 64) {
+            const float x = kth_max(p, a.row, r.top_k);
+            if (threadIdx.x == 0) p.bound[a.row] = fmaxf(x, kLowest);
+        }
+        return;
+    }
+    r = settings(p, a.row, row_max(p, a.row, part_s));
+    if (r.greedy) return;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const float low = r.below(kDepth);
     if (!r.filters()) {
@@ -262,8 +303,7 @@ __global__ __launch_bounds__(256) void sample_hist_kernel(SampleArgs p) {
             load8(a.z, t * kTile + 8 * lane, a.end, p.wide, z);
             u64 m = 0;
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
-                if (z[e] >= low) m += r.kept(r.depth(z[e]));
+            for (int e = 0; e < 8; ++e) m += r.kept_any(r.depth(z[e]));
             m = wave_sum64(m);
             if (lane == 0) p.tmass[static_cast<size_t>(a.row) * p.tiles + t] = m;
         }
@@ -278,16 +318,29 @@ __global__ __launch_bounds__(256) void sample_hist_kernel(SampleArgs p) {
     float z[8], next[8];
     load8(a.z, a.begin + 8 * threadIdx.x, a.end, p.wide, next);
     for (int i = a.begin + 8 * threadIdx.x; i < a.end; i += 8 * 256) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) z[e] = next[e];
-        load8(a.z, i + 8 * 256, a.end, p.wide, next);
+        bool any = false;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            if (!(z[e] >= low)) continue;
-            const double d = r.depth(z[e]);
-            if (d >= kDepth) continue;
-            if (r.top_k) atomicAdd(&cnt_s[r.bin(d)], 1u);
-            if (masses) atomicAdd(&mass_s[r.bin(d)], r.mass(d));
+            z[e] = next[e];
+            any |= z[e] >= low;
+        }
+        load8(a.z, i + 8 * 256, a.end, p.wide, next);
+        if (!__any(any)) continue;
+        // all eight side by side: the series is one long chain
+        double d[8];
+        u64 m[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) d[e] = fmin(r.depth(z[e]), kDepth);
+        if (masses) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) m[e] = r.mass_of(r.weight(d[e]));
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            if (d[e] >= kDepth) continue;
+            const int bin = r.bin(d[e]);
+            if (r.top_k) atomicAdd(&cnt_s[bin], 1u);
+            if (masses) atomicAdd(&mass_s[bin], m[e]);
         }
     }
     __syncthreads();
@@ -372,44 +425,23 @@ __device__ Borders borders(const SampleArgs& p, int row_, const Row& r, BorderSh
     return b;
 }
 
-// The k-th largest of the maxima of groups of tiles: at least k logits reach it.  A wave's work, bit by bit
-// from the top.
-__device__ float kth_max(const SampleArgs& p, int row, int k) {
-    const int lane = threadIdx.x & 63, per = p.group;
-    uint32_t v[kBound / 64];
-#pragma unroll
-    for (int i = 0; i < kBound / 64; ++i) {
-        float m = -INFINITY;
-        const int g = 64 * i + lane;
-        for (int t = g * per; t < min(p.tiles, (g + 1) * per); ++t) m = fmaxf(m, p.tmax[static_cast<size_t>(row) * p.tiles + t]);
-        const uint32_t b = __float_as_uint(m);
-        v[i] = b >> 31 ? ~b : b | 0x80000000u;  // ordered as the values
-    }
-    uint32_t x = 0;
-    for (int bit = 31; bit >= 0; --bit) {
-        const uint32_t y = x | 1u << bit;
-        int n = 0;
-#pragma unroll
-        for (int i = 0; i < kBound / 64; ++i) n += __popcll(__ballot(v[i] >= y));
-        if (n >= k) x = y;
-    }
-    return __uint_as_float(x >> 31 ? x & 0x7fffffffu : ~x);
-}
-
 template <class T>
 __global__ __launch_bounds__(256) void sample_list_kernel(SampleArgs p) {
     __shared__ float part_s[4];
     __shared__ BorderShared sh;
-    __shared__ u64 key_s[kList];
+    __shared__ int idx_s[kList];
     __shared__ int n_s, at_s;
     const Part<T> a = part_of<T>(p);
-    const Row r = settings(p, a.row, row_max(p, a.row, part_s));
-    if (r.greedy || !r.filters()) return;
+    Row r = settings(p, a.row, 0.f);
     Borders b{0, kBins, kBins, 0, 0, 0};
     float low;
+    if (!r.filters()) return;
     if (r.bounded(p)) {
-        low = fmaxf(r.below(kDepth), kth_max(p, a.row, r.top_k));
+        if (r.greedy) return;
+        low = p.bound[a.row];
     } else {
+        r = settings(p, a.row, row_max(p, a.row, part_s));
+        if (r.greedy) return;
         b = borders<256>(p, a.row, r, sh);
         const int last = b.k_bin < kBins ? b.k_bin : b.top;  // the last bin looked at
         low = r.below(fmin((last + 1) / kBinsPerUnit, kDepth));
@@ -430,29 +462,44 @@ __global__ __launch_bounds__(256) void sample_list_kernel(SampleArgs p) {
             any |= z[e] >= low;
         }
         load8(a.z, i + 4 * kTile, a.end, p.wide, next);
-        if (any) {
+        if (b.sure == 0) {
+            // nothing is kept unseen; the list may hold some past the border
+            if (any) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    if (z[e] >= low) {
+                        const int at = atomicAdd(&n_s, 1);
+                        if (at < kList) idx_s[at] = i + e;
+                    }
+            }
+            continue;
+        }
+        if (__any(any)) {
+            double d[8];
+            u64 w[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) d[e] = fmin(r.depth(z[e]), kDepth);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) w[e] = r.kept_any(d[e]);
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                if (!(z[e] >= low)) continue;
-                const double d = r.depth(z[e]);
-                if (d >= kDepth) continue;
-                const int bin = r.bin(d);
+                const int bin = r.bin(d[e]);
                 if (bin < b.sure) {
-                    m += r.kept(d);
-                } else if (bin <= b.top || bin == b.k_bin) {
+                    m += w[e];
+                } else if (d[e] < kDepth && (bin <= b.top || bin == b.k_bin)) {
                     const int at = atomicAdd(&n_s, 1);
-                    if (at < kList) key_s[at] = order_key(z[e], i + e);
+                    if (at < kList) idx_s[at] = i + e;
                 }
             }
         }
-        if (b.sure == 0) continue;  // nothing is kept unseen
         m = wave_sum64(m);
         if (lane == 0) p.tmass[row * p.tiles + t] = m;
     }
     __syncthreads();
     if (threadIdx.x == 0 && n_s) at_s = static_cast<int>(atomicAdd(&p.cnt[row * (kBins + 1) + kBins], static_cast<unsigned>(n_s)));
     __syncthreads();
-    for (int i = threadIdx.x; i < min(n_s, kList) && at_s + i < kList; i += 256) p.list[row * kList + at_s + i] = key_s[i];
+    for (int i = threadIdx.x; i < min(n_s, kList) && at_s + i < kList; i += 256) 
+        p.list[row * kList + at_s + i] = order_key(clean(static_cast<float>(a.z[idx_s[i]])), idx_s[i]);
 }
 
 struct PickShared {
@@ -485,21 +532,54 @@ __device__ u64 find_last(PickShared& sh, Each each, unsigned before_n, u64 befor
     __syncthreads();
     const int n_sub = sh.n;
     if (n_sub <= kRanked) {
-        if (static_cast<int>(threadIdx.x) < n_sub) {
-            const u64 key = sh.sub[threadIdx.x], m = sh.sub_w[threadIdx.x];
-            unsigned n = before_n;
-            u64 before = before_m;
-            for (int j = 0; j < n_sub; ++j) {
-                const bool less = sh.sub[j] < key;
-                n += less;
-                before += less ? sh.sub_w[j] : 0;
+        const int t = threadIdx.x;
+        if (n_sub <= kCounted) {
+            // few: each against every other
+            if (t < n_sub) {
+                const u64 key = sh.sub[t], m = sh.sub_w[t];
+                unsigned n = before_n;
+                u64 before = before_m;
+                for (int j = 0; j < n_sub; ++j) {
+                    const bool less = sh.sub[j] < key;
+                    n += less;
+                    before += less ? sh.sub_w[j] : 0;
+                }
+                const bool hit = want_n ? n + 1 == want_n
+                                        : static_cast<double>(before) < want_m && static_cast<double>(before + m) >= want_m;
+                if (hit) {
+                    sh.found_key = key;
+                    sh.found_upto = before + m;
+                }
             }
-            const bool hit = want_n ? n + 1 == want_n
-                                    : static_cast<double>(before) < want_m && static_cast<double>(before + m) >= want_m;
-            if (hit) {
-                sh.found_key = key;
-                sh.found_upto = before + m;
+            __syncthreads();
+            *upto = sh.found_upto;
+            return sh.found_key;
+        }
+        // in order (bitonic sort of the next power of two, a pair per thread), the masses before each
+        int size = 2 * kCounted;
+        while (size < n_sub) size *= 2;
+        if (t >= n_sub && t < size) sh.sub[t] = ~0ull, sh.sub_w[t] = 0;
+        for (int k = 2; k <= size; k *= 2)
+            for (int j = k / 2; j > 0; j /= 2) {
+                __syncthreads();
+                if (t < size / 2) {
+                    const int i = 2 * t - (t & (j - 1));
+                    const u64 x = sh.sub[i], y = sh.sub[i + j];
+                    if ((x > y) == ((i & k) == 0)) {
+                        const u64 wx = sh.sub_w[i];
+                        sh.sub[i] = y, sh.sub[i + j] = x;
+                        sh.sub_w[i] = sh.sub_w[i + j], sh.sub_w[i + j] = wx;
+                    }
+                }
             }
+        __syncthreads();
+        const u64 m = t < n_sub ? sh.sub_w[t] : 0;
+        const u64 upto_t = block_scan<kPick>(m, sh.part) + before_m;
+        const bool hit = want_n ? before_n + t + 1 == want_n
+                                : static_cast<double>(upto_t - m) < want_m && static_cast<double>(upto_t) >= want_m;
+        if (t < n_sub && hit) {
+            sh.found_key = sh.sub[t];
+            sh.found_upto = upto_t;
         }
         __syncthreads();
         *upto = sh.found_upto;
@@ -730,13 +810,13 @@ __global__ __launch_bounds__(kPick) void sample_pick_kernel(SampleArgs p) {
     }
 }
 
-// Logits of a workgroup: about 1024 workgroups for all rows, whole rounds of 256 threads x 8.
+// Logits of a workgroup: about 2048 workgroups for all rows, whole rounds of 256 threads x 8.
 int chunk_of(int rows, int V) {
-    const int64_t want = static_cast<int64_t>(rows) * V / 1024;
+    const int64_t want = static_cast<int64_t>(rows) * V / 2048;
     return static_cast<int>(std::max<int64_t>((want + 2047) / 2048, V / 512 / 2048 + 1)) * 2048;
 }
 struct SampleSpace {
-    size_t cmax, tmax, cnt, mass, tmass, list, bytes;
+    size_t cmax, tmax, bound, cnt, mass, tmass, list, bytes;
 };
 SampleSpace sample_space(int rows, int V, int chunks, int tiles) {
     SampleSpace s;
@@ -747,7 +827,8 @@ SampleSpace sample_space(int rows, int V, int chunks, int tiles) {
     s.cnt = s.list + n * kList * 8;
     s.cmax = s.cnt + n * (kBins + 1) * 4;
     s.tmax = s.cmax + n * chunks * 4;
-    s.bytes = (s.tmax + n * tiles * 4 + 255) / 256 * 256;
+    s.bound = s.tmax + n * tiles * 4;
+    s.bytes = (s.bound + n * 4 + 255) / 256 * 256;
     return s;
 }
 
@@ -803,6 +884,7 @@ void sample_rows(int dtype, const void* logits, int64_t ld, int rows, int V, con
     p.cnt = reinterpret_cast<unsigned*>(w + sp.cnt);
     p.cmax = reinterpret_cast<float*>(w + sp.cmax);
     p.tmax = reinterpret_cast<float*>(w + sp.tmax);
+    p.bound = reinterpret_cast<float*>(w + sp.bound);
     if (dtype == RL_Q_F32)
         launch_sample<float>(p, rows, s);
     else if (dtype == RL_Q_F16)

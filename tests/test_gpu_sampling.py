@@ -168,3 +168,30 @@ def test_the_same_from_call_to_call(gpu):
     a = [ops.sample_rows(z, u, temperature=1.2, top_p=0.95) for _ in range(3)]
     for b in a[1:]:
         assert np.array_equal(a[0][0], b[0]) and np.array_equal(a[0][1], b[1])
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_low_temperatures_and_far_apart_logits(gpu, dtype):
+    """Top-k reaches logits that weigh nothing, deep below the maximum; rows of which little is left
+    by a mask; more of top-k than logits above -infinity."""
+    z, u, r = rows(17, 8, 40000, std=3.0)
+    z[1, 300:] = -np.inf
+    z[2, 20:] = -np.inf
+    z[3] *= 1e4
+    z[4, 7:] = -np.inf
+    z[5] = np.where(r.random(40000) < 1e-3, z[5], -np.inf)
+    for t in (0.01, 1e-6, 1e-30, 1.0, 1e4, np.inf):
+        check(z, u, dtype, temperature=t, top_k=[50, 50, 50, 30, 10, 39, 700, 3000])
+        check(z, u, dtype, temperature=t, top_k=[50, 500, 20, 3000, 10, 39, 0, 1], top_p=0.9, min_p=0.01)
+        check(z, u, dtype, temperature=t, top_p=[0.5, 0.9, 0.99, 0.999, 0.1, 0.7, 0.3, 0.95])
+
+
+def test_most_likely_tokens_side_by_side(gpu):
+    """The largest logits in one run of indices: more of them in a tile than the tiles' maxima show."""
+    r = np.random.default_rng(19)
+    z = r.standard_normal((6, 248320)).astype(np.float32)
+    z[:, 70000:76000] += 20
+    u = r.random(6).astype(np.float32)
+    check(z, u, top_k=[1, 40, 200, 240, 1500, 5500])
+    check(z, u, top_k=[1, 40, 200, 240, 1500, 5500], top_p=0.9)
+    check(z, u, top_p=[0.9, 0.99, 0.5, 0.1, 0.999, 0.97])
