@@ -672,9 +672,9 @@ void launch_tree(const TreeArgs& p, int wp, hipStream_t s) {
     default: hipLaunchKernelGGL((tree_attn_kernel<R, HD, 4>), grid, dim3(256), 0, s, p); break;
     }
     check_launch("tree_attn_kernel");
-    // 4096 outputs: a wave each
+    // 512 outputs: a wave each
     const int64_t outs = static_cast<int64_t>(p.rows) * p.nq;
-    if (outs < 4096)
+    if (outs < 512)
         hipLaunchKernelGGL((tree_attn_join_kernel<R, HD, 4>), dim3(outs), dim3(256), 0, s, p, 32 * wp);
     else
         hipLaunchKernelGGL((tree_attn_join_kernel<R, HD, 1>), dim3((outs + 3) / 4), dim3(256), 0, s, p, 32 * wp);
