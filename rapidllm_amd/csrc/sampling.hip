@@ -91,22 +91,23 @@ __device__ inline void load8(const T* row, int i, int end, bool wide, float (&z)
     }
 }
 
-// 2^r for |r| <= 1/2, to 2^-50: the exponential's series to the 12th power
+// 2^r for |r| <= 1/2: the series of exp(r ln 2) to the 12th power, to 2^-50
 __device__ inline double exp2_small(double r) {
-    const double x = r * 0.693147180559945309417;
-    double y = 1.0 / 479001600.0;
-    y = fma(y, x, 1.0 / 39916800.0);
-    y = fma(y, x, 1.0 / 3628800.0);
-    y = fma(y, x, 1.0 / 362880.0);
-    y = fma(y, x, 1.0 / 40320.0);
-    y = fma(y, x, 1.0 / 5040.0);
-    y = fma(y, x, 1.0 / 720.0);
-    y = fma(y, x, 1.0 / 120.0);
-    y = fma(y, x, 1.0 / 24.0);
-    y = fma(y, x, 1.0 / 6.0);
-    y = fma(y, x, 0.5);
-    y = fma(y, x, 1.0);
-    return fma(y, x, 1.0);
+    constexpr double c = 0.693147180559945309417;
+    constexpr double c2 = c * c, c3 = c2 * c, c4 = c2 * c2, c5 = c4 * c, c6 = c3 * c3;
+    double y = c6 * c6 / 479001600.0;
+    y = fma(y, r, c6 * c5 / 39916800.0);
+    y = fma(y, r, c5 * c5 / 3628800.0);
+    y = fma(y, r, c5 * c4 / 362880.0);
+    y = fma(y, r, c4 * c4 / 40320.0);
+    y = fma(y, r, c4 * c3 / 5040.0);
+    y = fma(y, r, c6 / 720.0);
+    y = fma(y, r, c5 / 120.0);
+    y = fma(y, r, c4 / 24.0);
+    y = fma(y, r, c3 / 6.0);
+    y = fma(y, r, c2 / 2.0);
+    y = fma(y, r, c);
+    return fma(y, r, 1.0);
 }
 
 // A row's settings, and what its logits weigh.
@@ -131,27 +132,32 @@ struct Row {
         const double z = static_cast<double>(M) - depth / scale;
         return scale > 0.0 && z > -3e38 ? nextafterf(nextafterf(static_cast<float>(z), -INFINITY), -INFINITY) : kLowest;
     }
-    __device__ double weight(double depth) const {
-        const double n = rint(depth);
-        return ldexp(exp2_small(n - depth), -static_cast<int>(n));
+    // weight 2^-depth = p 2^-n for depths up to kDepth, and in units.  Adding 1.5 2^52 leaves a rounded number in
+    // a sum's low bits.
+    struct Weight {
+        double p;
+        int n;
+    };
+    __device__ static Weight weight(double depth) {
+        const double t = depth + 6755399441055744.0;
+        return {exp2_small((t - 6755399441055744.0) - depth), static_cast<int>(__double_as_longlong(t))};
     }
-    // 2^52 + w 2^shift holds the rounded number in its low bits
-    __device__ u64 mass_of(double w) const {
-        const double x = ldexp(w, shift) + 4503599627370496.0;
-        return static_cast<u64>(__double_as_longlong(x)) & 0xfffffffffffffull;
+    __device__ u64 mass_of(Weight w) const {
+        const double unit = __longlong_as_double(static_cast<long long>(1023 + shift - w.n) << 52);
+        return static_cast<u64>(__double_as_longlong(fma(w.p, unit, 4503599627370496.0))) & 0xfffffffffffffull;
     }
-    __device__ u64 mass(double depth) const { return depth < kDepth ? mass_of(weight(depth)) : 0; }
+    __device__ bool enough(Weight w) const {
+        return w.p * __longlong_as_double(static_cast<long long>(1023 - w.n) << 52) >= min_p;
+    }
+    __device__ u64 mass(double depth) const {
+        const u64 m = mass_of(weight(fmin(depth, kDepth)));
+        return depth < kDepth ? m : 0;
+    }
     // with min_p: nothing of what falls under it
     __device__ u64 kept(double depth) const {
-        if (depth >= kDepth) return 0;
-        const double w = weight(depth);
-        return w >= min_p ? mass_of(w) : 0;
-    }
-    // the same without a branch
-    __device__ u64 kept_any(double depth) const {
-        const double w = weight(fmin(depth, kDepth));
+        const Weight w = weight(fmin(depth, kDepth));
         const u64 m = mass_of(w);
-        return depth < kDepth && w >= min_p ? m : 0;
+        return depth < kDepth && enough(w) ? m : 0;
     }
     __device__ static int bin(double depth) { return static_cast<int>(fmin(depth, kDepth) * kBinsPerUnit); }
 };
@@ -262,9 +268,10 @@ __device__ float kth_max(const SampleArgs& p, int row, int k) {
     uint32_t v[kBound / 64];
 #pragma unroll
     for (int i = 0; i < kBound / 64; ++i) {
-        float m = -INFINITY;
         const int g = 64 * i + lane;
-        for (int t = g * per; t < min(p.tiles, (g + 1) * per); ++t) m = fmaxf(m, p.tmax[static_cast<size_t>(row) * p.tiles + t]);
+        float m = g * per < p.tiles ? p.tmax[static_cast<size_t>(row) * p.tiles + g * per] : -INFINITY;
+        for (int t = g * per + 1; per > 1 && t < min(p.tiles, (g + 1) * per); ++t)
+            m = fmaxf(m, p.tmax[static_cast<size_t>(row) * p.tiles + t]);
         const uint32_t b = __float_as_uint(m);
         v[i] = b >> 31 ? ~b : b | 0x80000000u;  // ordered as the values
     }
@@ -303,7 +310,7 @@ __global__ __launch_bounds__(256) void sample_hist_kernel(SampleArgs p) {
             load8(a.z, t * kTile + 8 * lane, a.end, p.wide, z);
             u64 m = 0;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) m += r.kept_any(r.depth(z[e]));
+            for (int e = 0; e < 8; ++e) m += r.kept(r.depth(z[e]));
             m = wave_sum64(m);
             if (lane == 0) p.tmass[static_cast<size_t>(a.row) * p.tiles + t] = m;
         }
@@ -430,6 +437,7 @@ __global__ __launch_bounds__(256) void sample_list_kernel(SampleArgs p) {
     __shared__ float part_s[4];
     __shared__ BorderShared sh;
     __shared__ int idx_s[kList];
+    __shared__ float2 few_s[4][kTile];
     __shared__ int n_s, at_s;
     const Part<T> a = part_of<T>(p);
     Row r = settings(p, a.row, 0.f);
@@ -450,48 +458,49 @@ __global__ __launch_bounds__(256) void sample_list_kernel(SampleArgs p) {
     const size_t row = a.row;
     if (threadIdx.x == 0) n_s = 0;
     __syncthreads();
-    float z[8], next[8];
-    load8(a.z, a.begin + wave * kTile + 8 * lane, a.end, p.wide, next);
     for (int t = a.begin / kTile + wave; t * kTile < a.end; t += 4) {
-        const int i = t * kTile + 8 * lane;
-        u64 m = 0;
-        bool any = false;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            z[e] = next[e];
-            any |= z[e] >= low;
-        }
-        load8(a.z, i + 4 * kTile, a.end, p.wide, next);
-        if (b.sure == 0) {
-            // nothing is kept unseen; the list may hold some past the border
-            if (any) {
-#pragma unroll
-                for (int e = 0; e < 8; ++e)
-                    if (z[e] >= low) {
-                        const int at = atomicAdd(&n_s, 1);
-                        if (at < kList) idx_s[at] = i + e;
-                    }
-            }
+        // a tile whose maximum does not reach it
+        if (!(p.tmax[row * p.tiles + t] >= low)) {
+            if (b.sure && lane == 0) p.tmass[row * p.tiles + t] = 0;
             continue;
         }
-        if (__any(any)) {
-            double d[8];
-            u64 w[8];
+        const int i = t * kTile + 8 * lane;
+        float z[8];
+        load8(a.z, i, a.end, p.wide, z);
+        if (b.sure == 0) {
+            // nothing is kept unseen; the list may hold some past the border
 #pragma unroll
-            for (int e = 0; e < 8; ++e) d[e] = fmin(r.depth(z[e]), kDepth);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) w[e] = r.kept_any(d[e]);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const int bin = r.bin(d[e]);
-                if (bin < b.sure) {
-                    m += w[e];
-                } else if (d[e] < kDepth && (bin <= b.top || bin == b.k_bin)) {
+            for (int e = 0; e < 8; ++e)
+                if (z[e] >= low) {
                     const int at = atomicAdd(&n_s, 1);
                     if (at < kList) idx_s[at] = i + e;
                 }
+            continue;
+        }
+        // what reaches it, close together: few of a tile do
+        int n = 0;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const unsigned long long mask = __ballot(z[e] >= low);
+            const int at = n + __builtin_amdgcn_mbcnt_hi(mask >> 32, __builtin_amdgcn_mbcnt_lo(mask, 0));
+            if (z[e] >= low) few_s[wave][at] = make_float2(z[e], __int_as_float(i + e));
+            n += __popcll(mask);
+        }
+        __builtin_amdgcn_wave_barrier();
+        u64 m = 0;
+        for (int k = lane; k < n; k += 64) {
+            const float2 x = few_s[wave][k];
+            const double d = r.depth(x.x);
+            const int bin = r.bin(d);
+            const u64 w = r.kept(d);
+            if (bin < b.sure) {
+                m += w;
+            } else if (d < kDepth && (bin <= b.top || bin == b.k_bin)) {
+                const int at = atomicAdd(&n_s, 1);
+                if (at < kList) idx_s[at] = __float_as_int(x.y);
             }
         }
+        __builtin_amdgcn_wave_barrier();
         m = wave_sum64(m);
         if (lane == 0) p.tmass[row * p.tiles + t] = m;
     }
