@@ -436,8 +436,9 @@ template <class T>
 __global__ __launch_bounds__(256) void sample_list_kernel(SampleArgs p) {
     __shared__ float part_s[4];
     __shared__ BorderShared sh;
-    __shared__ int idx_s[kList];
-    __shared__ float2 few_s[4][kTile];
+    __shared__ uint16_t idx_s[kList];  // within the chunk
+    __shared__ float few_s[4][kTile];
+    __shared__ uint16_t few_i[4][kTile];
     __shared__ int n_s, at_s;
     const Part<T> a = part_of<T>(p);
     Row r = settings(p, a.row, 0.f);
@@ -458,22 +459,28 @@ __global__ __launch_bounds__(256) void sample_list_kernel(SampleArgs p) {
     const size_t row = a.row;
     if (threadIdx.x == 0) n_s = 0;
     __syncthreads();
-    for (int t = a.begin / kTile + wave; t * kTile < a.end; t += 4) {
-        // a tile whose maximum does not reach it
-        if (!(p.tmax[row * p.tiles + t] >= low)) {
-            if (b.sure && lane == 0) p.tmass[row * p.tiles + t] = 0;
-            continue;
-        }
-        const int i = t * kTile + 8 * lane;
+    // the wave's tiles (at most 32), one per lane: those whose maximum reaches it
+    const int t0 = a.begin / kTile + wave, mine = t0 + 4 * lane;
+    const bool have = mine * kTile < a.end;
+    const bool reach = have && p.tmax[row * p.tiles + mine] >= low;
+    if (b.sure && have && !reach) p.tmass[row * p.tiles + mine] = 0;
+    unsigned long long todo = __ballot(reach);
+    float next[8];
+    if (todo) load8(a.z, (t0 + 4 * (__ffsll(todo) - 1)) * kTile + 8 * lane, a.end, p.wide, next);
+    while (todo) {
+        const int t = t0 + 4 * (__ffsll(todo) - 1), i = t * kTile + 8 * lane;
+        todo &= todo - 1;
         float z[8];
-        load8(a.z, i, a.end, p.wide, z);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) z[e] = next[e];
+        if (todo) load8(a.z, (t0 + 4 * (__ffsll(todo) - 1)) * kTile + 8 * lane, a.end, p.wide, next);
         if (b.sure == 0) {
             // nothing is kept unseen; the list may hold some past the border
 #pragma unroll
             for (int e = 0; e < 8; ++e)
                 if (z[e] >= low) {
                     const int at = atomicAdd(&n_s, 1);
-                    if (at < kList) idx_s[at] = i + e;
+                    if (at < kList) idx_s[at] = static_cast<uint16_t>(i + e - a.begin);
                 }
             continue;
         }
@@ -483,21 +490,23 @@ __global__ __launch_bounds__(256) void sample_list_kernel(SampleArgs p) {
         for (int e = 0; e < 8; ++e) {
             const unsigned long long mask = __ballot(z[e] >= low);
             const int at = n + __builtin_amdgcn_mbcnt_hi(mask >> 32, __builtin_amdgcn_mbcnt_lo(mask, 0));
-            if (z[e] >= low) few_s[wave][at] = make_float2(z[e], __int_as_float(i + e));
+            if (z[e] >= low) {
+                few_s[wave][at] = z[e];
+                few_i[wave][at] = static_cast<uint16_t>(i + e - a.begin);
+            }
             n += __popcll(mask);
         }
         __builtin_amdgcn_wave_barrier();
         u64 m = 0;
         for (int k = lane; k < n; k += 64) {
-            const float2 x = few_s[wave][k];
-            const double d = r.depth(x.x);
+            const double d = r.depth(few_s[wave][k]);
             const int bin = r.bin(d);
             const u64 w = r.kept(d);
             if (bin < b.sure) {
                 m += w;
             } else if (d < kDepth && (bin <= b.top || bin == b.k_bin)) {
                 const int at = atomicAdd(&n_s, 1);
-                if (at < kList) idx_s[at] = __float_as_int(x.y);
+                if (at < kList) idx_s[at] = few_i[wave][k];
             }
         }
         __builtin_amdgcn_wave_barrier();
@@ -507,8 +516,10 @@ __global__ __launch_bounds__(256) void sample_list_kernel(SampleArgs p) {
     __syncthreads();
     if (threadIdx.x == 0 && n_s) at_s = static_cast<int>(atomicAdd(&p.cnt[row * (kBins + 1) + kBins], static_cast<unsigned>(n_s)));
     __syncthreads();
-    for (int i = threadIdx.x; i < min(n_s, kList) && at_s + i < kList; i += 256) 
-        p.list[row * kList + at_s + i] = order_key(clean(static_cast<float>(a.z[idx_s[i]])), idx_s[i]);
+    for (int i = threadIdx.x; i < min(n_s, kList) && at_s + i < kList; i += 256) {
+        const int at = a.begin + idx_s[i];
+        p.list[row * kList + at_s + i] = order_key(clean(static_cast<float>(a.z[at])), at);
+    }
 }
 
 struct PickShared {
@@ -529,8 +540,8 @@ struct PickShared {
 
 // Which of the elements that `each` hands out ends the prefix: the one with `want_n` up to it (before_n stand
 // before all of them), or else the first up to which want_m of mass stands.  The key of it, *upto the mass up to it.
-template <class Each>
-__device__ u64 find_last(PickShared& sh, Each each, unsigned before_n, u64 before_m, unsigned want_n, double want_m, u64* upto) {
+template <class Each, class Mass>
+__device__ u64 find_last(PickShared& sh, Mass mass, Each each, unsigned before_n, u64 before_m, unsigned want_n, double want_m, u64* upto) {
     __syncthreads();
     if (threadIdx.x == 0) sh.n = 0;
     __syncthreads();
@@ -564,30 +575,29 @@ __device__ u64 find_last(PickShared& sh, Each each, unsigned before_n, u64 befor
             *upto = sh.found_upto;
             return sh.found_key;
         }
-        // in order (bitonic sort of the next power of two, a pair per thread), the masses before each
-        int size = 2 * kCounted;
-        while (size < n_sub) size *= 2;
-        if (t >= n_sub && t < size) sh.sub[t] = ~0ull, sh.sub_w[t] = 0;
-        for (int k = 2; k <= size; k *= 2)
+        // in order (bitonic sort, a key per thread: partners of the same wave by lane moves), the masses before each
+        u64 key = t < n_sub ? sh.sub[t] : ~0ull;
+        for (int k = 2; k <= kRanked; k *= 2) {
             for (int j = k / 2; j > 0; j /= 2) {
-                __syncthreads();
-                if (t < size / 2) {
-                    const int i = 2 * t - (t & (j - 1));
-                    const u64 x = sh.sub[i], y = sh.sub[i + j];
-                    if ((x > y) == ((i & k) == 0)) {
-                        const u64 wx = sh.sub_w[i];
-                        sh.sub[i] = y, sh.sub[i + j] = x;
-                        sh.sub_w[i] = sh.sub_w[i + j], sh.sub_w[i + j] = wx;
-                    }
+                u64 other;
+                if (j >= 64) {
+                    __syncthreads();
+                    sh.sub[t] = key;
+                    __syncthreads();
+                    other = sh.sub[t ^ j];
+                } else {
+                    other = __shfl_xor(key, j, 64);
                 }
+                const bool least = ((t & j) == 0) == ((t & k) == 0);
+                key = (key < other) == least ? key : other;
             }
-        __syncthreads();
-        const u64 m = t < n_sub ? sh.sub_w[t] : 0;
+        }
+        const u64 m = t < n_sub ? mass(key) : 0;
         const u64 upto_t = block_scan<kPick>(m, sh.part) + before_m;
         const bool hit = want_n ? before_n + t + 1 == want_n
                                 : static_cast<double>(upto_t - m) < want_m && static_cast<double>(upto_t) >= want_m;
         if (t < n_sub && hit) {
-            sh.found_key = sh.sub[t];
+            sh.found_key = key;
             sh.found_upto = upto_t;
         }
         __syncthreads();
@@ -632,6 +642,10 @@ __global__ __launch_bounds__(kPick) void sample_pick_kernel(SampleArgs p) {
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const size_t row = blockIdx.x;
     const T* zr = static_cast<const T*>(p.logits) + row * p.ld;
+    // asked for before they are known to be there
+    const u64 first = p.list[row * kList + tid];
+    const unsigned n_all = p.cnt[row * (kBins + 1) + kBins];
+    const float u0 = p.u[row];
     const Row r = settings(p, row, row_max(p, row, sh.fpart));
     if (r.greedy) {
         // the first chunk with the maximum, its first such logit
@@ -660,13 +674,13 @@ __global__ __launch_bounds__(kPick) void sample_pick_kernel(SampleArgs p) {
     int n_list = 0;
     int sure = kBins;  // bins before it are in the tiles' masses
     if (r.filters()) {
-        const unsigned n = p.cnt[row * (kBins + 1) + kBins];
-        listed = n <= kList;
-        n_list = listed ? n : 0;
+        listed = n_all <= kList;
+        n_list = listed ? n_all : 0;
         for (int i = tid; i < n_list; i += kPick) {
-            sh.key[i] = p.list[row * kList + i];
+            sh.key[i] = i < kPick ? first : p.list[row * kList + i];
             sh.w[i] = r.mass(r.depth(key_value(sh.key[i])));
         }
+        const auto mass_of = [&](u64 key) { return r.mass(r.depth(key_value(key))); };
         // the elements of some bins with keys up to one: from the list, or where that is too short from the row
         const auto each_of = [&](int bin_lo, int bin_hi, u64 upto, auto f) {
             if (listed) {
@@ -725,7 +739,7 @@ __global__ __launch_bounds__(kPick) void sample_pick_kernel(SampleArgs p) {
                 }
                 __syncthreads();
                 k_bin = sh.bin;
-                last = find_last(sh, [&](auto f) { each_of(k_bin, k_bin, ~0ull, f); }, sh.before_n, sh.before_m, r.top_k, 0.0, &left);
+                last = find_last(sh, mass_of, [&](auto f) { each_of(k_bin, k_bin, ~0ull, f); }, sh.before_n, sh.before_m, r.top_k, 0.0, &left);
             }
             if (r.use_p) {
                 const double want = fmax(r.top_p * static_cast<double>(left), 0.5);
@@ -744,14 +758,14 @@ __global__ __launch_bounds__(kPick) void sample_pick_kernel(SampleArgs p) {
                 __syncthreads();
                 const int p_bin = sh.bin;
                 u64 upto;
-                last = find_last(sh, [&](auto f) { each_of(p_bin, p_bin, last, f); }, 0, sh.before_m, 0, want, &upto);
+                last = find_last(sh, mass_of, [&](auto f) { each_of(p_bin, p_bin, last, f); }, 0, sh.before_m, 0, want, &upto);
             }
         } else {
             const Borders b = borders<kPick>(p, row, r, sh.b);
             sure = b.sure;
             u64 left = b.all, before = 0;
             if (b.k_bin < kBins)
-                last = find_last(sh, [&](auto f) { each_of(b.k_bin, b.k_bin, ~0ull, f); }, b.k_before, b.k_mass, r.top_k, 0.0, &left);
+                last = find_last(sh, mass_of, [&](auto f) { each_of(b.k_bin, b.k_bin, ~0ull, f); }, b.k_before, b.k_mass, r.top_k, 0.0, &left);
             if (r.use_p) {
                 // the bins from b.sure to b.top hold the border; the mass before them
                 const double want = fmax(r.top_p * static_cast<double>(left), 0.5);
@@ -759,7 +773,7 @@ __global__ __launch_bounds__(kPick) void sample_pick_kernel(SampleArgs p) {
                 for (int i = tid; i < b.sure; i += kPick) m += p.mass[row * kBins + i];
                 block_scan<kPick>(m, sh.part, &before);
                 u64 upto;
-                last = find_last(sh, [&](auto f) { each_of(b.sure, b.top, last, f); }, 0, before, 0, want, &upto);
+                last = find_last(sh, mass_of, [&](auto f) { each_of(b.sure, b.top, last, f); }, 0, before, 0, want, &upto);
             }
         }
         __syncthreads();
@@ -792,7 +806,6 @@ __global__ __launch_bounds__(kPick) void sample_pick_kernel(SampleArgs p) {
     const u64 mine = sh.range[tid];
     u64 total;
     const u64 upto = block_scan<kPick>(mine, sh.part, &total);
-    const float u0 = p.u[row];
     const double target = static_cast<double>(u0 >= 0.f ? fminf(u0, 0.99999994f) : 0.f) * static_cast<double>(total);
     if (mine && static_cast<double>(upto - mine) <= target && static_cast<double>(upto) > target) {
         sh.at = tid;
@@ -819,10 +832,10 @@ __global__ __launch_bounds__(kPick) void sample_pick_kernel(SampleArgs p) {
     }
 }
 
-// Logits of a workgroup: about 2048 workgroups for all rows, whole rounds of 256 threads x 8.
+// Logits of a workgroup: about 2048 workgroups for all rows, whole rounds of 256 threads x 8, up to 65536.
 int chunk_of(int rows, int V) {
     const int64_t want = static_cast<int64_t>(rows) * V / 2048;
-    return static_cast<int>(std::max<int64_t>((want + 2047) / 2048, V / 512 / 2048 + 1)) * 2048;
+    return static_cast<int>(std::min<int64_t>(std::max<int64_t>((want + 2047) / 2048, V / 512 / 2048 + 1), 32)) * 2048;
 }
 struct SampleSpace {
     size_t cmax, tmax, bound, cnt, mass, tmass, list, bytes;
