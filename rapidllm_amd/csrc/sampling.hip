@@ -29,7 +29,7 @@ constexpr int kTile = 512;             // logits of a wave at a time, 8 per lane
 constexpr int kBins = 2048;
 constexpr double kBinsPerUnit = 44.0;  // bins of depth
 constexpr double kDepth = 45.0;        // weights from 2^-45 down are no unit
-constexpr int kList = 4096;            // elements of the border bins that are listed
+constexpr int kList = 3000;            // elements of the border bins that are listed
 constexpr float kLowest = -3.40282347e38f;
 constexpr int kSmallK = 2048;
 constexpr int kBound = 512;            // maxima that a wave finds the k-th largest of
@@ -74,7 +74,7 @@ __device__ inline float clean(float z) {
     z += 0.f;
     return z != z ? -INFINITY : z;
 }
-// logits i .. i + 7, -infinity past the row
+// logits i .. i + 7 as they are (NaN passes no comparison), -infinity past the row
 template <class T>
 __device__ inline void load8(const T* row, int i, int end, bool wide, float (&z)[8]) {
     if (wide && i + 8 <= end) {
@@ -83,11 +83,11 @@ __device__ inline void load8(const T* row, int i, int end, bool wide, float (&z)
         for (int k = 0; k < 8; k += 16 / sizeof(T)) {
             const T8 v = *reinterpret_cast<const T8*>(row + i + k);
 #pragma unroll
-            for (unsigned e = 0; e < 16 / sizeof(T); ++e) z[k + e] = clean(static_cast<float>(v[e]));
+            for (unsigned e = 0; e < 16 / sizeof(T); ++e) z[k + e] = static_cast<float>(v[e]);
         }
     } else {
 #pragma unroll
-        for (int k = 0; k < 8; ++k) z[k] = i + k < end ? clean(static_cast<float>(row[i + k])) : -INFINITY;
+        for (int k = 0; k < 8; ++k) z[k] = i + k < end ? static_cast<float>(row[i + k]) : -INFINITY;
     }
 }
 
@@ -123,7 +123,7 @@ struct Row {
     // (M - z) / (T ln 2), >= 0; past kDepth for what has no weight at all
     __device__ double depth(float z) const {
         if (z == M) return 0.0;
-        if (z == -INFINITY || M == INFINITY) return 1e9;
+        if (!(z > -INFINITY) || M == INFINITY) return 1e9;
         return (static_cast<double>(M) - static_cast<double>(z)) * scale;
     }
     // everything below it lies deeper (two steps of z down, for the rounding); never -infinity
@@ -157,7 +157,7 @@ struct Row {
     __device__ u64 kept(double depth) const {
         const Weight w = weight(fmin(depth, kDepth));
         const u64 m = mass_of(w);
-        return depth < kDepth && enough(w) ? m : 0;
+        return depth < kDepth && (min_p == 0.0 || enough(w)) ? m : 0;
     }
     __device__ static int bin(double depth) { return static_cast<int>(fmin(depth, kDepth) * kBinsPerUnit); }
 };
@@ -437,8 +437,7 @@ __global__ __launch_bounds__(256) void sample_list_kernel(SampleArgs p) {
     __shared__ float part_s[4];
     __shared__ BorderShared sh;
     __shared__ uint16_t idx_s[kList];  // within the chunk
-    __shared__ float few_s[4][kTile];
-    __shared__ uint16_t few_i[4][kTile];
+    __shared__ float2 few_s[4][kTile];  // logit, place in the chunk
     __shared__ int n_s, at_s;
     const Part<T> a = part_of<T>(p);
     Row r = settings(p, a.row, 0.f);
@@ -485,28 +484,32 @@ __global__ __launch_bounds__(256) void sample_list_kernel(SampleArgs p) {
             continue;
         }
         // what reaches it, close together: few of a tile do
-        int n = 0;
+        int own = 0;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const unsigned long long mask = __ballot(z[e] >= low);
-            const int at = n + __builtin_amdgcn_mbcnt_hi(mask >> 32, __builtin_amdgcn_mbcnt_lo(mask, 0));
-            if (z[e] >= low) {
-                few_s[wave][at] = z[e];
-                few_i[wave][at] = static_cast<uint16_t>(i + e - a.begin);
-            }
-            n += __popcll(mask);
+        for (int e = 0; e < 8; ++e) own += z[e] >= low;
+        int upto = own;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const int x = __shfl_up(upto, o, 64);
+            upto += lane >= o ? x : 0;
         }
+        const int n = __builtin_amdgcn_readlane(upto, 63);
+        int at = upto - own;
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            if (z[e] >= low) few_s[wave][at++] = make_float2(z[e], __int_as_float(i + e - a.begin));
         __builtin_amdgcn_wave_barrier();
         u64 m = 0;
         for (int k = lane; k < n; k += 64) {
-            const double d = r.depth(few_s[wave][k]);
+            const float2 x = few_s[wave][k];
+            const double d = r.depth(x.x);
             const int bin = r.bin(d);
             const u64 w = r.kept(d);
             if (bin < b.sure) {
                 m += w;
             } else if (d < kDepth && (bin <= b.top || bin == b.k_bin)) {
-                const int at = atomicAdd(&n_s, 1);
-                if (at < kList) idx_s[at] = few_i[wave][k];
+                const int to = atomicAdd(&n_s, 1);
+                if (to < kList) idx_s[to] = static_cast<uint16_t>(__float_as_int(x.y));
             }
         }
         __builtin_amdgcn_wave_barrier();
