@@ -374,8 +374,11 @@ int rl_hip_paged_append(const RlPagedCache* cache, int layer, int dtype, const v
  * multiple of n_kv with at most 64 query heads per kv head; max_rows: no sequence has
  * more rows (rows past it are left out).  A context that with its rows passes the table
  * is cut to what the table holds; a page number outside the cache is read as page 0.
- * q and gate aligned and strided as in rl_hip_paged_append; out 16-byte aligned.
- * workspace: rl_hip_tree_attn_workspace_bytes; calls that overlap in time need one each. */
+ * q and gate aligned and strided as in rl_hip_paged_append; out 16-byte aligned, mask 8.
+ * Half-precision rows multiply in their type (the weights rounded to it, 32-bit sums);
+ * RL_Q_F32 rows as two half-precision parts, to about 2^-21: their q below 65504.
+ * workspace: rl_hip_tree_attn_workspace_bytes (one made for more rows serves fewer); calls
+ * that overlap in time need one each. */
 size_t rl_hip_tree_attn_workspace_bytes(int n_q, int n_kv, int head_dim, int n_seq, int max_rows);
 int rl_hip_tree_attn(const RlPagedCache* cache, int layer, int dtype, const void* q, int64_t q_row, int64_t q_head,
                      const void* gate, int64_t gate_row, int64_t gate_head, const int* table, int table_width,

@@ -659,8 +659,9 @@ Split split_of(int nq, int nkv, int hd, int max_rows) {
 size_t tree_attn_workspace_bytes(int nq, int nkv, int hd, int n_seq, int max_rows) {
     (void)n_seq;
     if (nq < 1 || nkv < 1 || nq % nkv || hd < 1 || max_rows < 1) return 256;
+    // at least what split_of takes, and never less for more rows: a workspace serves every smaller max_rows
     const Split s = split_of(nq, nkv, hd, max_rows);
-    return static_cast<size_t>(s.workers) * s.q_tiles * 2 * 32 * s.wp * (hd * 4 + 8) + 256;
+    return static_cast<size_t>(std::max(kSlots(hd), 8 * s.q_tiles)) * 2 * 32 * s.wp * (hd * 4 + 8) + 256;
 }
 
 template <class R, int HD>
@@ -701,7 +702,7 @@ void tree_attn(const RlPagedCache* c, int layer, int dtype, const void* q, int64
                "tree_attn: n_q must be a multiple of n_kv, at most 64 per kv head");
     RL_REQUIRE(width >= 1 && static_cast<int64_t>(width) * c->page_size <= INT32_MAX, RL_ERR_RANGE,
                "tree_attn: bad table width");
-    RL_REQUIRE(!mask || words >= 1, RL_ERR_RANGE, "tree_attn: a mask needs words");
+    RL_REQUIRE(!mask || (words >= 1 && aligned(mask, 8)), RL_ERR_RANGE, "tree_attn: a mask needs words, 8-byte aligned");
     RL_REQUIRE(scale > -INFINITY && scale < INFINITY, RL_ERR_RANGE, "tree_attn: bad scale");
     if (rows == 0 || n_seq == 0 || max_rows == 0) return;
     RL_REQUIRE(q && table && ctx_lens && row_start && out && ws, RL_ERR_RANGE, "tree_attn: null pointer");
@@ -713,7 +714,7 @@ void tree_attn(const RlPagedCache* c, int layer, int dtype, const void* q, int64
                RL_ERR_UNSUPPORTED, "tree_attn: more than 2^31 units of work");
     RL_REQUIRE(static_cast<int64_t>(c->n_pages) * c->n_kv * c->page_size <= UINT32_MAX, RL_ERR_UNSUPPORTED,
                "tree_attn: a layer's cache has more than 2^32 rows");
-    RL_REQUIRE(ws_bytes >= tree_attn_workspace_bytes(nq, c->n_kv, c->head_dim, n_seq, max_rows), RL_ERR_RANGE,
+    RL_REQUIRE(ws_bytes >= tree_attn_workspace_bytes(nq, c->n_kv, c->head_dim, n_seq, std::min(max_rows, rows)), RL_ERR_RANGE,
                "tree_attn: workspace too small");
     TreeArgs p{};
     p.q = q, p.gate = gate;
@@ -726,7 +727,7 @@ void tree_attn(const RlPagedCache* c, int layer, int dtype, const void* q, int64
     p.nq = nq, p.nkv = c->n_kv, p.page = c->page_size, p.n_pages = c->n_pages;
     p.scale = scale, p.out = out;
     while ((1 << p.page_log2) < c->page_size) ++p.page_log2;
-    const Split sp = split_of(nq, c->n_kv, c->head_dim, max_rows);
+    const Split sp = split_of(nq, c->n_kv, c->head_dim, std::min(max_rows, rows));
     p.q_tiles = sp.q_tiles, p.workers = sp.workers, p.unit = unit_of(sp.wp);
     const size_t parts = static_cast<size_t>(sp.workers) * sp.q_tiles * 2 * 32 * sp.wp;
     p.part_o = static_cast<float*>(ws);

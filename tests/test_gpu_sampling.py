@@ -195,3 +195,38 @@ def test_most_likely_tokens_side_by_side(gpu):
     check(z, u, top_k=[1, 40, 200, 240, 1500, 5500])
     check(z, u, top_k=[1, 40, 200, 240, 1500, 5500], top_p=0.9)
     check(z, u, top_p=[0.9, 0.99, 0.5, 0.1, 0.999, 0.97])
+
+
+@pytest.mark.parametrize("V", [(1 << 20) + 3, 3000001])
+def test_large_vocabularies(gpu, V):
+    """Groups of several tiles, shares of several tiles per thread; coarser units."""
+    r = np.random.default_rng(V)
+    z = (r.standard_normal((3, V)) * 2).astype(np.float32)
+    z[:, r.integers(0, V, 50)] += 9
+    u = r.random(3).astype(np.float32)
+    for kw in (dict(), dict(top_k=[40, 300, 3000]), dict(top_p=[0.9, 0.5, 0.99]), dict(temperature=0.0)):
+        idx, prob = ops.sample_rows(z, u, **kw)
+        for i in range(3):
+            g = {a: np.broadcast_to(v, (3,))[i] for a, v in kw.items()}
+            want, pr, room = plain(z[i], u[i], g.get("temperature", 1.0), int(g.get("top_k", 0)),
+                                   np.float32(g.get("top_p", 1.0)))
+            # half a unit (vocab 2^-63) a token
+            if want != idx[i] and 0 < room < V * V * 2.0 ** -63:
+                continue
+            assert idx[i] == want, (kw, i, room)
+            assert abs(prob[i] - pr) <= 2.0 ** -20 * pr + V * 2.0 ** -62
+
+
+def test_without_probabilities(gpu):
+    """out_prob may be NULL, and so may every setting."""
+    from rapidllm_amd import hip
+    from rapidllm_amd.hip import DeviceBuffer, call
+
+    z, u, _ = rows(23, 4, 5000)
+    d, du, di = DeviceBuffer.from_numpy(z), DeviceBuffer.from_numpy(u), DeviceBuffer(16)
+    t = DeviceBuffer.from_numpy(np.array([1, 0, 1, 0], np.float32))
+    ws = DeviceBuffer(hip.lib().rl_hip_sample_workspace_bytes(4, 5000))
+    call("rl_hip_sample_rows", F32, d.ptr, 5000, 4, 5000, t.ptr, None, None, None, du.ptr, di.ptr, None, ws.ptr,
+         ws.nbytes, None)
+    got = di.numpy(np.int32, (4,))
+    assert got.tolist() == [plain(z[i], u[i], [1, 0, 1, 0][i])[0] for i in range(4)]

@@ -139,3 +139,18 @@ def test_workspace_sizes(L):
     assert a[0] > 0 and a == sorted(a)
     s = [L.rl_hip_sample_workspace_bytes(r, v) for r, v in ((1, 1000), (1, 248320), (128, 248320))]
     assert s[0] > 0 and s == sorted(s)
+
+
+def test_attn_mask_alignment_and_size_limits(L):
+    assert attn(L, cache(), mask=P + 4, words=1) == RANGE
+    # more rows than 32-bit row numbers hold, more units of work than 32 bits count
+    big = cache(n_pages=1 << 20, page_size=4096, layer_stride=0)
+    assert attn(L, big) == UNSUPPORTED
+    assert attn(L, cache(), width=(1 << 27) - 1, n_seq=4000) == UNSUPPORTED
+
+
+@pytest.mark.parametrize("nq,nkv,hd", [(24, 4, 256), (32, 8, 128), (64, 1, 64)])
+def test_attn_workspace_serves_fewer_rows(L, nq, nkv, hd):
+    """Non-decreasing over max_rows, so that one workspace serves every smaller step."""
+    a = [L.rl_hip_tree_attn_workspace_bytes(nq, nkv, hd, 8, r) for r in range(1, 700)]
+    assert a == sorted(a)
