@@ -308,52 +308,49 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void tree_attn_kernel(TreeA
             for (int v = 0; v < 16; ++v) o[dt][v] = 0.f;
         float m = -INFINITY, l = 0.f;
 
-        // S^T = K . Q^T of the tiles, in log2 units
-        auto scores = [&](const i32x4* Kt, f32x16 (&sn)[NT]) {
+        // S^T = K . Q^T of a tile, in log2 units; side(i): what is done under product i of HD / 16
+        auto scores = [&](const i32x4* Kt, f32x16& sn, auto side) {
             const char* K = reinterpret_cast<const char*>(Kt);
             const int own = opaque(kaddr);
 #pragma unroll
-            for (int a = 0; a < NT; ++a)
-#pragma unroll
-                for (int v = 0; v < 16; ++v) sn[a][v] = 0.f;
-            // product i: dims 16 (i / NT), tile i % NT; its K read kAhead products before
-            constexpr int N = NT * HD / 16;
-            auto read = [&](int i) { return *reinterpret_cast<const i32x4*>(K + (own ^ 32 * (i / NT)) + (i % NT) * kTile * 16); };
+            for (int v = 0; v < 16; ++v) sn[v] = 0.f;
+            // dims 16 i; their K read kAhead products before
+            constexpr int N = HD / 16;
+            auto read = [&](int i) { return *reinterpret_cast<const i32x4*>(K + (own ^ 32 * i)); };
             i32x4 kk[kAhead];
 #pragma unroll
             for (int i = 0; i < kAhead; ++i) kk[i] = read(i);
 #pragma unroll
             for (int i = 0; i < N; ++i) {
-                sn[i % NT] = F::mfma(kk[i % kAhead], qh[i / NT], sn[i % NT]);
-                if constexpr (kTwo) sn[i % NT] = F::mfma(kk[i % kAhead], ql[i / NT], sn[i % NT]);
-                pin(sn[i % NT]);
+                sn = F::mfma(kk[i % kAhead], qh[i], sn);
+                if constexpr (kTwo) sn = F::mfma(kk[i % kAhead], ql[i], sn);
+                pin(sn);
                 if (i + kAhead < N) kk[i % kAhead] = read(i + kAhead);
+                side(i);
                 __builtin_amdgcn_sched_barrier(0);
             }
-#pragma unroll
-            for (int a = 0; a < NT; ++a) sn[a] *= sc;
+            sn *= sc;
         };
+        const auto nothing = [](int) {};
         auto hide = [&](f32x16& sn, uint32_t vis) {
 #pragma unroll
             for (int v = 0; v < 16; ++v)
                 if (!(vis >> (8 * (v >> 2) + 4 * h + (v & 3)) & 1)) sn[v] = -INFINITY;
         };
-        // the running maximum follows the scores once one passes it by kRaise
-        auto raise = [&](f32x16 (&sn)[NT]) {
-            float mx = -INFINITY;
+        // the running maximum follows the scores once one passes it by kRaise; true where it did
+        auto raise = [&](const f32x16& sn) {
+            float mx = sn[0];
 #pragma unroll
-            for (int a = 0; a < NT; ++a)
-#pragma unroll
-                for (int v = 0; v < 16; ++v) mx = fmaxf(mx, sn[a][v]);
+            for (int v = 1; v < 16; ++v) mx = fmaxf(mx, sn[v]);
             mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-            if (__any(mx > m + kRaise)) {
-                const float mn = fmaxf(m, mx);
-                const float alpha = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
-                m = mn;
-                l *= alpha;
+            if (!__any(mx > m + kRaise)) return false;
+            const float mn = fmaxf(m, mx);
+            const float alpha = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+            m = mn;
+            l *= alpha;
 #pragma unroll
-                for (int dt = 0; dt < HD / 32; ++dt) o[dt] *= alpha;
-            }
+            for (int dt = 0; dt < HD / 32; ++dt) o[dt] *= alpha;
+            return true;
         };
         struct Weights {
             typename F::type hi[2], lo[kTwo ? 2 : 1];
@@ -448,7 +445,7 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void tree_attn_kernel(TreeA
             auto rounds = [&]<bool edge>(std::bool_constant<edge> e, int from, int to) {
                 for (int u = from; u < to; ++u) {
                     const bool more = u + 1 < ub, runs = page_runs && u + 1 < u_edge;
-                    f32x16 sn[1];
+                    f32x16 sn;
                     uint32_t vis = ~0u;
                     Weights w;
                     // all but the last kLoads loads, V's
@@ -456,18 +453,18 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void tree_attn_kernel(TreeA
                     const uint32_t rows = row_of(next, min(u + 1, ub - 1), wave);
                     next = page_of(min(u + 2, ub - 1), wave);
                     asm volatile("" ::: "memory");
-                    scores(K, sn);
+                    scores(K, sn, nothing);
                     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
                     if (more) load(p.k, K, rows, false, runs);
-                    if constexpr (edge) hide(sn[0], vis = seen32(p, s, j, u * kUnit + 32 * wave));
+                    if constexpr (edge) hide(sn, vis = seen32(p, s, j, u * kUnit + 32 * wave));
                     raise(sn);
-                    weights(sn[0], w, level());
+                    weights(sn, w, level());
                     // all but the next K's
                     if (more)
                         asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kLoads) : "memory");
                     else
                         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-                    output(e, V, w, vis, [](int) {});
+                    output(e, V, w, vis, nothing);
                     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
                     if (more) load(p.v, V, rows, true, runs);
                 }
@@ -490,29 +487,49 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void tree_attn_kernel(TreeA
                     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
                     const uint32_t rows = row_of(next, min(u + 1, ub - 1), wave & 1);
                     next = page_of(min(u + 2, ub - 1), wave & 1);
-                    if (u + 1 < ub) load(pool, mem + ((u + 1) & 1) * 2 * kTile, rows, is_v, page_runs && u + 1 < u_edge);
                     const i32x4 *K = K_s + ((u & 1) * 2 + ws * NT) * kTile, *V = V_s + ((u & 1) * 2 + ws * NT) * kTile;
+                    i32x4* to = mem + ((u + 1) & 1) * 2 * kTile;
                     f32x16 sn[NT];
                     uint32_t vis[NT];
                     Weights w[NT];
-                    scores(K, sn);
 #pragma unroll
-                    for (int a = 0; a < NT; ++a) {
-                        vis[a] = ~0u;
-                        if constexpr (edge) hide(sn[a], vis[a] = seen32(p, s, j, u * kUnit + 32 * (ws * NT + a)));
+                    for (int a = 0; a < NT; ++a) vis[a] = ~0u;
+                    // the next round's loads under the first tile's scores
+                    if (u + 1 < ub && page_runs && u + 1 < u_edge) {
+                        const int own = own_offset(is_v);
+                        scores(K, sn[0], [&](int i) {
+                            if (i < kLoads) load1(pool, to, rows, is_v, true, own, i);
+                        });
+                    } else {
+                        if (u + 1 < ub) load(pool, to, rows, is_v, false);
+                        scores(K, sn[0], nothing);
                     }
-                    raise(sn);
-                    const float sub = level();
-                    weights(sn[0], w[0], sub);
+                    if constexpr (edge) hide(sn[0], vis[0] = seen32(p, s, j, u * kUnit + 32 * ws * NT));
+                    raise(sn[0]);
                     if constexpr (NT == 2) {
-                        // the second tile's weights under the first one's products
+                        // the first tile's weights under the second one's scores, the second one's under the
+                        // first one's output
+                        float sub = level();
+                        scores(K + kTile, sn[1], [&](int i) {
+#pragma unroll
+                            for (int k = 8 * i / (HD / 16); k < 8 * (i + 1) / (HD / 16); ++k) weights2(sn[0], w[0], sub, k);
+                        });
+                        if constexpr (edge) hide(sn[1], vis[1] = seen32(p, s, j, u * kUnit + 32 * (ws * NT + 1)));
+                        if (raise(sn[1])) {
+                            // rarely: the first tile's weights once more, their sum is in l
+                            const float had = l;
+                            sub = level();
+                            weights(sn[0], w[0], sub);
+                            l = had;
+                        }
                         output(e, V, w[0], vis[0], [&](int i) {
 #pragma unroll
                             for (int k = 8 * i / (HD / 16); k < 8 * (i + 1) / (HD / 16); ++k) weights2(sn[1], w[1], sub, k);
                         });
-                        output(e, V + kTile, w[1], vis[1], [](int) {});
+                        output(e, V + kTile, w[1], vis[1], nothing);
                     } else {
-                        output(e, V, w[0], vis[0], [](int) {});
+                        weights(sn[0], w[0], level());
+                        output(e, V, w[0], vis[0], nothing);
                     }
                 }
             };
