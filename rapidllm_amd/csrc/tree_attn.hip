@@ -164,6 +164,14 @@ __device__ inline int opaque(int v) {
     return v;
 }
 
+// Waits for all but the last kVm loads from memory, or all but kLds shared-memory reads (63, 15: for none).
+// Builtins, not asm: the compiler then knows what is still on its way, and waits for single reads after it.
+template <int kVm, int kLds>
+__device__ inline void wait() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt((kVm & 15) | (kVm >> 4) << 14 | 7 << 4 | kLds << 8);
+    asm volatile("" ::: "memory");
+}
 // Keeps a product where it stands among the reads and the vector work (the compiler sinks it to its use).
 __device__ inline void pin(f32x16& v) { asm volatile("" : "+v"(v)); }
 
@@ -238,37 +246,41 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void tree_attn_kernel(TreeA
             return ((static_cast<uint32_t>(pg) * static_cast<uint32_t>(p.nkv) + kv) << p.page_log2) +
                    (min(u * kUnit + 32 * k + col, L - 1) & (p.page - 1));
         };
-        // Load i of a tile: kPerLoad rows.  Where they lie in one page (`runs`), their address is a scalar and
-        // a lane's offset; else, and for rows past the last position, each row's own.
-        auto load1 = [&](const void* pool, i32x4* dst, uint32_t rows, bool is_v, bool runs, int own, int i) {
-            const char* src;
-            if (runs) {
+        // Load i of a tile: kPerLoad rows.  Where they lie in one page (`runs`), their address is a scalar (in a
+        // buffer resource) and a lane's offset; else, and for rows past the last position, each row's own.
+        // Global loads to shared memory count as both kinds of access: while one may be on its way, the compiler
+        // waits for every read.  They stay out of the loop that most rounds run in.
+        auto load1 = [&]<bool runs>(std::bool_constant<runs>, const void* pool, i32x4* dst, uint32_t rows, bool is_v, int own, int i) {
+            if constexpr (runs) {
                 const int f = is_v ? v_swap<HD>(i * kPerLoad) : k_swap<HD>(i * kPerLoad);
                 const uint32_t r0 = __builtin_amdgcn_readlane(rows, i * kPerLoad);
-                src = static_cast<const char*>(pool) + static_cast<size_t>(r0) * (U * 16) + static_cast<uint32_t>(own ^ f * 16);
+                char* src = static_cast<char*>(const_cast<void*>(pool)) + static_cast<size_t>(r0) * (U * 16);
+                const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(src, 0, 1024, 0x00020000);
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_void*)(dst + i * 64), 16, own ^ f * 16, 0, 0, 0);
             } else {
                 const int r = i * kPerLoad + own / (U * 16), u = lane % U;
                 const int f = is_v ? v_swap<HD>(r) : k_swap<HD>(r);
                 const uint32_t at = __shfl(rows, r, 64);
-                src = static_cast<const char*>(pool) + (static_cast<size_t>(at) * U + (u ^ f)) * 16;
+                const char* src = static_cast<const char*>(pool) + (static_cast<size_t>(at) * U + (u ^ f)) * 16;
+                __builtin_amdgcn_global_load_lds((global_void*)src, (lds_void*)(dst + i * 64), 16, 0, 0);
             }
-            __builtin_amdgcn_global_load_lds((global_void*)src, (lds_void*)(dst + i * 64), 16, 0, 0);
         };
         // a lane's offset within a load's rows: the swaps of rows i * kPerLoad + lane / U are those of the two parts, xor
         auto own_offset = [&](bool is_v) {
             const int r = lane / U, f = is_v ? v_swap<HD>(r) : k_swap<HD>(r);
             return opaque(r * U * 16 + ((lane % U) ^ f) * 16);
         };
-        auto load = [&](const void* pool, i32x4* dst, uint32_t rows, bool is_v, bool runs) {
+        auto load_of = [&]<bool runs>(std::bool_constant<runs> r, const void* pool, i32x4* dst, uint32_t rows, bool is_v) {
             const int own = own_offset(is_v);
             rows = opaque(rows);
-            if (runs) {
 #pragma unroll
-                for (int i = 0; i < kLoads; ++i) load1(pool, dst, rows, is_v, true, own, i);
-            } else {
-#pragma unroll
-                for (int i = 0; i < kLoads; ++i) load1(pool, dst, rows, is_v, false, own, i);
-            }
+            for (int i = 0; i < kLoads; ++i) load1(r, pool, dst, rows, is_v, own, i);
+        };
+        auto load = [&](const void* pool, i32x4* dst, uint32_t rows, bool is_v, bool runs) {
+            if (runs)
+                load_of(std::true_type(), pool, dst, rows, is_v);
+            else
+                load_of(std::false_type(), pool, dst, rows, is_v);
         };
         const bool page_runs = p.page >= kPerLoad;
 
@@ -436,7 +448,7 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void tree_attn_kernel(TreeA
             }
         };
         // rounds up to u_edge hold positions of the context alone
-        const int u_edge = min(max(s.ctx / kUnit, ua), ub);
+        const int u_edge = min(max(s.ctx / kUnit, ua), ub), u_runs = page_runs ? max(u_edge - 1, ua) : ua;
         if constexpr (WP == 1) {
             // every wave by itself: K of its next tile comes while this one's V is used, and the other way round
             i32x4 *K = K_s + wave * kTile, *V = V_s + wave * kTile;
@@ -449,35 +461,37 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void tree_attn_kernel(TreeA
                 load(p.v, V, rows, true, page_runs && ua < u_edge);
             }
             split_q();
-            auto rounds = [&]<bool edge>(std::bool_constant<edge> e, int from, int to) {
+            // runs: the next round's loads are runs of rows, and there is a next round
+            auto rounds = [&]<bool edge, bool runs>(std::bool_constant<edge> e, std::bool_constant<runs> r, int from, int to) {
                 for (int u = from; u < to; ++u) {
-                    const bool more = u + 1 < ub, runs = page_runs && u + 1 < u_edge;
+                    const bool more = runs || u + 1 < ub;
                     f32x16 sn;
                     uint32_t vis = ~0u;
                     Weights w;
                     // all but the last kLoads loads, V's
-                    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kLoads) : "memory");
+                    wait<kLoads, 15>();
                     const uint32_t rows = row_of(next, min(u + 1, ub - 1), wave);
                     next = page_of(min(u + 2, ub - 1), wave);
                     asm volatile("" ::: "memory");
                     scores(K, sn, nothing);
-                    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-                    if (more) load(p.k, K, rows, false, runs);
+                    wait<63, 0>();
+                    if (more) load_of(r, p.k, K, rows, false);
                     if constexpr (edge) hide(sn, vis = seen32(p, s, j, u * kUnit + 32 * wave));
                     raise(sn);
                     weights(sn, w, level());
                     // all but the next K's
                     if (more)
-                        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kLoads) : "memory");
+                        wait<kLoads, 15>();
                     else
-                        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+                        wait<0, 15>();
                     output(e, V, w, vis, nothing);
-                    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-                    if (more) load(p.v, V, rows, true, runs);
+                    wait<63, 0>();
+                    if (more) load_of(r, p.v, V, rows, true);
                 }
             };
-            rounds(std::false_type(), ua, u_edge);
-            rounds(std::true_type(), u_edge, ub);
+            rounds(std::false_type(), std::true_type(), ua, u_runs);
+            rounds(std::false_type(), std::false_type(), u_runs, u_edge);
+            rounds(std::true_type(), std::false_type(), u_edge, ub);
         } else {
             // wave w brings tile w % 2 of K (w < 2) or V: the next round's while this one is computed
             const bool is_v = wave >= 2;
@@ -489,9 +503,11 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void tree_attn_kernel(TreeA
                 next = page_of(min(ua + 1, ub - 1), wave & 1);
             }
             split_q();
-            auto rounds = [&]<bool edge>(std::bool_constant<edge> e, int from, int to) {
+            auto rounds = [&]<bool edge, bool runs>(std::bool_constant<edge> e, std::bool_constant<runs> r, int from, int to) {
                 for (int u = from; u < to; ++u) {
-                    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+                    wait<0, 0>();
+                    __builtin_amdgcn_s_barrier();
+                    asm volatile("" ::: "memory");
                     const uint32_t rows = row_of(next, min(u + 1, ub - 1), wave & 1);
                     next = page_of(min(u + 2, ub - 1), wave & 1);
                     const i32x4 *K = K_s + ((u & 1) * 2 + ws * NT) * kTile, *V = V_s + ((u & 1) * 2 + ws * NT) * kTile;
@@ -502,13 +518,13 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void tree_attn_kernel(TreeA
 #pragma unroll
                     for (int a = 0; a < NT; ++a) vis[a] = ~0u;
                     // the next round's loads under the first tile's scores
-                    if (u + 1 < ub && page_runs && u + 1 < u_edge) {
+                    if constexpr (runs) {
                         const int own = own_offset(is_v);
                         scores(K, sn[0], [&](int i) {
-                            if (i < kLoads) load1(pool, to, rows, is_v, true, own, i);
+                            if (i < kLoads) load1(r, pool, to, rows, is_v, own, i);
                         });
                     } else {
-                        if (u + 1 < ub) load(pool, to, rows, is_v, false);
+                        if (u + 1 < ub) load_of(r, pool, to, rows, is_v);
                         scores(K, sn[0], nothing);
                     }
                     if constexpr (edge) hide(sn[0], vis[0] = seen32(p, s, j, u * kUnit + 32 * ws * NT));
@@ -540,8 +556,9 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void tree_attn_kernel(TreeA
                     }
                 }
             };
-            rounds(std::false_type(), ua, u_edge);
-            rounds(std::true_type(), u_edge, ub);
+            rounds(std::false_type(), std::true_type(), ua, u_runs);
+            rounds(std::false_type(), std::false_type(), u_runs, u_edge);
+            rounds(std::true_type(), std::false_type(), u_edge, ub);
         }
         l += __shfl_xor(l, 32, 64);
 
