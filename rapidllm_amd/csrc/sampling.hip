@@ -544,6 +544,21 @@ struct PickShared {
     int digit, n, at, bin;
 };
 
+// How many of n keys are less than `key`, and their masses; the arrays are filled up to a multiple of 8 with
+// ~0 (eight at a time are read side by side).
+__device__ inline void count_less(const u64* keys, const u64* w, int n, u64 key, unsigned* less, u64* mass) {
+    for (int j = 0; j < n; j += 8) {
+        u64 k[8], m[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) k[e] = keys[j + e], m[e] = w[j + e];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            *less += k[e] < key;
+            *mass += k[e] < key ? m[e] : 0;
+        }
+    }
+}
+
 // Which of the elements that `each` hands out ends the prefix: the one with `want_n` up to it (before_n stand
 // before all of them), or else the first up to which want_m of mass stands.  The key of it, *upto the mass up to it.
 template <class Each, class Mass>
@@ -561,15 +576,13 @@ __device__ u64 find_last(PickShared& sh, Mass mass, Each each, unsigned before_n
         const int t = threadIdx.x;
         if (n_sub <= kCounted) {
             // few: each against every other
+            if (t >= n_sub && t < n_sub + 8) sh.sub[t] = ~0ull, sh.sub_w[t] = 0;
+            __syncthreads();
             if (t < n_sub) {
                 const u64 key = sh.sub[t], m = sh.sub_w[t];
                 unsigned n = before_n;
                 u64 before = before_m;
-                for (int j = 0; j < n_sub; ++j) {
-                    const bool less = sh.sub[j] < key;
-                    n += less;
-                    before += less ? sh.sub_w[j] : 0;
-                }
+                count_less(sh.sub, sh.sub_w, n_sub, key, &n, &before);
                 const bool hit = want_n ? n + 1 == want_n
                                         : static_cast<double>(before) < want_m && static_cast<double>(before + m) >= want_m;
                 if (hit) {
@@ -707,7 +720,25 @@ __global__ __launch_bounds__(kPick) void sample_pick_kernel(SampleArgs p) {
                 }
             }
         };
-        if (r.small_k()) {
+        if (r.small_k() && listed && n_list <= kCounted) {
+            // few: each against every other gives both borders
+            sure = 0;
+            if (tid == 0) sh.found_key = 0, sh.found_upto = 0;
+            if (tid >= n_list && tid < n_list + 8) sh.key[tid] = ~0ull, sh.w[tid] = 0;
+            __syncthreads();
+            u64 key = 0, before = 0;
+            unsigned rank = 0;
+            if (tid < n_list) {
+                key = sh.key[tid];
+                count_less(sh.key, sh.w, n_list, key, &rank, &before);
+                if (rank + 1 == static_cast<unsigned>(min(r.top_k, n_list))) sh.found_upto = before + sh.w[tid];
+            }
+            __syncthreads();
+            const double want = fmax(r.top_p * static_cast<double>(sh.found_upto), 0.5);
+            if (tid < n_list && rank < static_cast<unsigned>(r.top_k) && (!r.use_p || static_cast<double>(before) < want)) atomicMax(&sh.found_key, key);
+            __syncthreads();
+            if (n_list) last = sh.found_key;
+        } else if (r.small_k()) {
             // a histogram of the list, top-k's border in it, then top-p's in what that leaves
             sure = 0;
             for (int i = tid; i < kBins; i += kPick) sh.cnt[i] = 0, sh.mass[i] = 0;
