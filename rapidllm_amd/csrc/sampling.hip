@@ -13,8 +13,8 @@
 // border bins' elements; the choice.  Up to kSmallK, all that top-k may keep goes to the list and the
 // histogram needs no masses; where there are 2 k tiles (or groups of them) it is not needed at all: the k-th
 // largest of their maxima is a bound that at least k elements reach, and few others do.  One workgroup per row
-// doing all of it took 344 us for one row of 248320 logits, 633 us for 128; now 24 us (the launches and the
-// last one's chain of small steps, 12 us) and 116 us.  128 rows with top-k: 21 us for the one pass
+// doing all of it took 344 us for one row of 248320 logits, 633 us for 128; now 22 us (the launches and the
+// last one's chain of small steps, 10 us) and 102 to 117 us.  128 rows with top-k: 21 us for the one pass
 // over 127 MB of logits (6 TB/s), 31 us after it; with top-p alone 150 us, bound by the 64-bit arithmetic
 // of the weights (about 24 such instructions a logit, twice for the ones that are kept).
 #include <algorithm>
