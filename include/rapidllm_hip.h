@@ -346,7 +346,7 @@ int rl_hip_accept_prefix(const int* toks, const int* preds, int T, int* pos, int
  * row_start[n_seq] on belong to none and their outputs are left as they were), a
  * context of ctx_lens[b] positions, and its row j sits at position ctx_lens[b] + j of
  * its page table (entry p / page_size of row b of `table` [n_seq][table_width]; entries
- * past the sequence's last position are not read).
+ * past the sequence's last position are not read; table_width * page_size <= 2^30).
  * `dtype` is the rows' type: RL_Q_F32 (over an RL_Q_F16 cache) or the cache's own.
  * Lengths, tables and slots are read on the device, so a captured call follows them;
  * page numbers and slots outside the cache are never accessed. */

@@ -37,6 +37,8 @@ __device__ inline void store4(T* p, f32x4 v) {
     *reinterpret_cast<typename Vec4<T>::type*>(p) = o;
 }
 
+constexpr int64_t kMaxPositions = 1 << 30;  // of a table's row: sums of two stay in 32 bits
+
 // A sequence of a step: rows r0 .. r0 + n - 1, context ctx.  Whatever the arrays hold, the rows
 // stay within 0 .. rows and the positions within the table's capacity.
 struct SeqSpan {

@@ -232,7 +232,7 @@ void tree_accept(const RlPagedCache* c, const int* table, int width, const int* 
     RL_REQUIRE(cap >= 1 && cap <= kPathCap, RL_ERR_RANGE, "tree_accept: path_cap must be in 1..4096");
     if (c) {
         check_cache(c, 0, "tree_accept");
-        RL_REQUIRE(width >= 1 && static_cast<int64_t>(width) * c->page_size <= INT32_MAX, RL_ERR_RANGE,
+        RL_REQUIRE(width >= 1 && static_cast<int64_t>(width) * c->page_size <= kMaxPositions, RL_ERR_RANGE,
                    "tree_accept: bad table width");
     }
     if (n_seq == 0) return;

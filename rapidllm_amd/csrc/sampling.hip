@@ -241,9 +241,9 @@ __global__ __launch_bounds__(256) void sample_max_kernel(SampleArgs p) {
     for (int t = a.begin / kTile + wave; t * kTile < a.end; t += 4) {
         float z[8];
         load8(a.z, t * kTile + 8 * lane, a.end, p.wide, z);
-        float x = z[0];
+        float x = -INFINITY;  // also of a tile of NaN
 #pragma unroll
-        for (int e = 1; e < 8; ++e) x = fmaxf(x, z[e]);
+        for (int e = 0; e < 8; ++e) x = fmaxf(x, z[e]);
         x = wave_max(x);
         m = fmaxf(m, x);
         if (lane == 0) p.tmax[static_cast<size_t>(a.row) * p.tiles + t] = x;

@@ -743,7 +743,7 @@ void tree_attn(const RlPagedCache* c, int layer, int dtype, const void* q, int64
     RL_REQUIRE(rows >= 0 && n_seq >= 0 && max_rows >= 0, RL_ERR_RANGE, "tree_attn: bad sizes");
     RL_REQUIRE(nq >= 1 && nq % c->n_kv == 0 && nq / c->n_kv <= kMaxGroup, RL_ERR_RANGE,
                "tree_attn: n_q must be a multiple of n_kv, at most 64 per kv head");
-    RL_REQUIRE(width >= 1 && static_cast<int64_t>(width) * c->page_size <= INT32_MAX, RL_ERR_RANGE,
+    RL_REQUIRE(width >= 1 && static_cast<int64_t>(width) * c->page_size <= kMaxPositions, RL_ERR_RANGE,
                "tree_attn: bad table width");
     RL_REQUIRE(!mask || (words >= 1 && aligned(mask, 8)), RL_ERR_RANGE, "tree_attn: a mask needs words, 8-byte aligned");
     RL_REQUIRE(scale > -INFINITY && scale < INFINITY, RL_ERR_RANGE, "tree_attn: bad scale");
@@ -752,9 +752,9 @@ void tree_attn(const RlPagedCache* c, int layer, int dtype, const void* q, int64
     check_strided(q, q_row, q_head, dtype, "tree_attn");
     if (gate) check_strided(gate, gate_row, gate_head, dtype, "tree_attn");
     RL_REQUIRE(aligned(out, 16) && aligned(ws, 16), RL_ERR_RANGE, "tree_attn: out and workspace must be 16-byte aligned");
-    RL_REQUIRE(static_cast<double>(n_seq) * c->n_kv * (static_cast<double>(width) * c->page_size / 64 + 1) < INT32_MAX &&
+    RL_REQUIRE(static_cast<double>(n_seq) * c->n_kv * (static_cast<double>(width) * c->page_size / 64 + 1) < (1 << 30) &&
                    static_cast<int64_t>(rows) * nq < INT32_MAX,
-               RL_ERR_UNSUPPORTED, "tree_attn: more than 2^31 units of work");
+               RL_ERR_UNSUPPORTED, "tree_attn: more than 2^30 units of work");
     RL_REQUIRE(static_cast<int64_t>(c->n_pages) * c->n_kv * c->page_size <= UINT32_MAX, RL_ERR_UNSUPPORTED,
                "tree_attn: a layer's cache has more than 2^32 rows");
     RL_REQUIRE(ws_bytes >= tree_attn_workspace_bytes(nq, c->n_kv, c->head_dim, n_seq, std::min(max_rows, rows)), RL_ERR_RANGE,

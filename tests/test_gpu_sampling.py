@@ -230,3 +230,18 @@ def test_without_probabilities(gpu):
          ws.nbytes, None)
     got = di.numpy(np.int32, (4,))
     assert got.tolist() == [plain(z[i], u[i], [1, 0, 1, 0][i])[0] for i in range(4)]
+
+
+def test_runs_of_nan(gpu):
+    """Whole stretches of a row are NaN: they count for nothing, also where maxima of stretches decide."""
+    z, u, r = rows(29, 6, 60000)
+    z[0, 512:1024] = np.nan
+    z[1, :4096] = np.nan
+    z[2, 10000:] = np.nan
+    z[3, r.random(60000) < 0.9] = np.nan
+    z[4, 1:] = np.nan
+    for k in (1, 2, 5, 40):
+        check(z, u, top_k=k)
+        check(z, u, F16, top_k=k, top_p=0.9)
+    check(z, u, top_p=0.95)
+    check(z, u)

@@ -146,7 +146,7 @@ def test_attn_mask_alignment_and_size_limits(L):
     # more rows than 32-bit row numbers hold, more units of work than 32 bits count
     big = cache(n_pages=1 << 20, page_size=4096, layer_stride=0)
     assert attn(L, big) == UNSUPPORTED
-    assert attn(L, cache(), width=(1 << 27) - 1, n_seq=4000) == UNSUPPORTED
+    assert attn(L, cache(), width=1 << 26, n_seq=4000) == UNSUPPORTED
 
 
 @pytest.mark.parametrize("nq,nkv,hd", [(24, 4, 256), (32, 8, 128), (64, 1, 64)])
@@ -154,3 +154,8 @@ def test_attn_workspace_serves_fewer_rows(L, nq, nkv, hd):
     """Non-decreasing over max_rows, so that one workspace serves every smaller step."""
     a = [L.rl_hip_tree_attn_workspace_bytes(nq, nkv, hd, 8, r) for r in range(1, 700)]
     assert a == sorted(a)
+
+
+def test_tables_of_more_than_2_30_positions(L):
+    assert attn(L, cache(), width=(1 << 26) + 1) == RANGE
+    assert accept(L, cache(), width=(1 << 26) + 1) == RANGE
