@@ -229,6 +229,16 @@ def test_tree_attn(gpu, dtype, nq, nkv, hd, page, ctx, rows, kind):
     assert np.array_equal(got, s.run(mask, gate))  # the same from call to call
 
 
+@pytest.mark.parametrize("hd,nq,nkv,rows", [(64, 4, 2, 3), (64, 12, 1, 5), (128, 8, 2, 9), (128, 8, 1, 20),
+                                            (256, 4, 1, 2), (256, 6, 1, 10), (256, 6, 1, 30)])
+@pytest.mark.parametrize("page", [1, 2, 4, 8, 32])
+def test_small_pages_under_long_contexts(gpu, hd, nq, nkv, rows, page):
+    """Every way a tile's rows are found, over many tiles: each row by itself, runs of rows, whole tiles."""
+    s = Step(page + hd, F16 if page % 4 else F32, nq, nkv, hd, page, [1900, 130, 1500], [rows, 1, rows])
+    mask = s.tree_mask()
+    agree(s.run(mask), *s.want(mask, False))
+
+
 @pytest.mark.parametrize("dtype", [F32, BF16])
 def test_rows_that_see_nothing(gpu, dtype):
     """A mask without a bit: zeros where the context is empty too, the context alone where not."""
