@@ -682,6 +682,8 @@ __global__ __launch_bounds__(256) void tree_attn_join_kernel(TreeArgs p, int til
 constexpr int kSlots(int hd) { return hd == 256 ? 256 : 512; }
 
 // Tiles of 32 pairs per workgroup: as many as a sequence's rows fill, the positions shared by the other waves.
+// 8 sequences x 16000 positions, 24 / 4 heads of 256, f32 / f16 rows: 24 pairs with 1, 2, 4 tiles 122 / 110, 127 / 109,
+// 172 / 116 us; 54 pairs with 2 and 4 131 / 118, 164 / 124 us.
 int pair_waves(int G, int max_rows) {
     const int64_t pairs = static_cast<int64_t>(G) * max_rows;
     return pairs <= 32 ? 1 : pairs <= 64 ? 2 : 4;
