@@ -37,8 +37,7 @@ constexpr float kLowest = -3.40282347e38f;
 constexpr int kSmallK = 2048;
 constexpr int kBound = 512;            // maxima that a wave finds the k-th largest of
 constexpr int kRanked = 1024;          // elements that are sorted in shared memory
-constexpr int kCounted = 128;          // ... that are put in order by counting the ones before each (60: 1 us, a
-                                       // sort 4; 1000: 55 us, a sort 5)
+constexpr int kCounted = 128;          // ... that are put in order by counting the ones before each
 constexpr int kPick = 1024;            // threads of the last launch
 
 struct SampleArgs {
@@ -871,7 +870,7 @@ __global__ __launch_bounds__(kPick) void sample_pick_kernel(SampleArgs p) {
 }
 
 // Logits of a workgroup: about 2048 workgroups for all rows, whole rounds of 256 threads x 8, up to 65536.
-// 128 rows of 248320, mixed settings / top-p / top-k and top-p: 1024 workgroups 142 / 148 / 51 us, 2048 119 / 145 / 57,
+// 128 rows of 248320, mixed settings / top-p / top-k and top-p: 1024 workgroups 142 / 147 / 51 us, 2048 119 / 145 / 57,
 // 4096 110 / 156 / 58 (every workgroup adds its bins to the row's histogram).
 int chunk_of(int rows, int V) {
     const int64_t want = static_cast<int64_t>(rows) * V / 2048;
