@@ -12,9 +12,10 @@
 // exact; sums, maxima and outputs in 32 bits.  Half-precision rows round the weights to their type,
 // as their output is rounded anyway.
 // Few pairs (up to 32): bound by HBM.  Every wave streams tiles of its own without a barrier; 1 row
-// x 131071 positions, 24 / 4 heads of 256: 537 MB in 95 us, 5.7 TB/s.  Many pairs: bound by the matrix cores;
+// x 131071 positions, 24 / 4 heads of 256: 537 MB in 97 us, 5.5 TB/s.  Many pairs: bound by the matrix cores;
 // 128 pairs share each K and V, 8 x 64 rows x 32000 positions of 32-bit rows: 0.81 PFLOP (in two
-// parts) in 767 us, 1.05 PFLOP/s where a large fp16 library product reaches 1.14.  Short contexts: bound by the
+// parts) in 785 us with the join, calls back to back, 1.03 PFLOP/s where a large fp16 library product reaches
+// 1.14 (ten launches under a trace: kernel 765 us at least, 932 median).  Short contexts: bound by the
 // chain of dependent loads and the instructions of one round; 1 row x 700 positions 13 + 4 us.  One
 // thread per dim and a wave per position, without MFMA: 134 us, 31.4 ms and 57 ms for these three.
 #include <algorithm>
